@@ -4,7 +4,7 @@ A case is a dict of plain values; ``kind`` names the operator and its direction:
 
   scan       h_t = a_t h_{t-1} + u_t over a sequence, from a carried state; a = sigmoid(gate) or the gate itself,
              u = (1 - a) x ("leaky") or x
-  scan_bwd   its gradients from the gradient of h
+  scan_train the same forward pass and then its gradients from the gradient of h
   norm       r' = r + alpha * s * act(gate) * rms_norm(y), z = rms_norm(r'): the norm behind one block, its gate and
              residual scale, and the norm in front of the next block
   norm_bwd   its gradients
@@ -37,8 +37,8 @@ def listed():
         # a padded batch of odd sizes in the framework's own order (time outermost), ready-made decays
         dict(name="scan_ragged_t1031_fp32", kind="scan", dtype="fp32", T=1031, B=6, D=1001, gate="value", leaky=False,
              batch_first=False, ragged=True, carry=True),
-        # training backward of the second case
-        dict(name="scan_bwd_t2048_b8_bf16", kind="scan_bwd", dtype="bf16", T=2048, B=8, D=2048, gate="sigmoid",
+        # training: forward and backward pass of the second case
+        dict(name="scan_train_t2048_b8_bf16", kind="scan_train", dtype="bf16", T=2048, B=8, D=2048, gate="sigmoid",
              leaky=True, batch_first=True, ragged=False, carry=False),
         # decode: norm, gate and residual between two blocks for four users
         dict(name="norm_m4_bf16", kind="norm", dtype="bf16", M=4, D=4096, gate="silu", post=True, pre=True),
@@ -64,9 +64,9 @@ def _log_int(rng, lo, hi):
 
 
 def _drawn(rng):
-    kind = rng.choice(["scan", "scan", "scan_bwd", "norm", "norm_bwd", "w4", "w4"])
+    kind = rng.choice(["scan", "scan", "scan_train", "norm", "norm_bwd", "w4", "w4"])
     c = dict(kind=kind, dtype=rng.choice(["bf16", "bf16", "fp16", "fp32"]))
-    if kind in ("scan", "scan_bwd"):
+    if kind in ("scan", "scan_train"):
         c["T"] = _log_int(rng, 1, 32768 if kind == "scan" else 8192)
         c["B"] = _log_int(rng, 1, 64)
         c["D"] = _log_int(rng, 64, 8192)
@@ -127,7 +127,7 @@ def prepare(case, seed):
         return (torch.randn(shape, generator=gen, device=dev) * std + mean).to(dtype)
 
     s = dict(case=case)
-    if case["kind"] in ("scan", "scan_bwd"):
+    if case["kind"] in ("scan", "scan_train"):
         T, B, D = case["T"], case["B"], case["D"]
         lead = (B, T) if case["batch_first"] else (T, B)
         if case["gate"] == "sigmoid":       # input and gate logits are the two halves of one projection's rows
@@ -142,15 +142,9 @@ def prepare(case, seed):
         if case["ragged"]:
             steps = torch.tensor(_steps(case), device=dev, dtype=torch.int32)
             s["lengths"] = steps[torch.randperm(B, generator=gen, device=dev)].contiguous()
-        if case["kind"] == "scan_bwd":
+        if case["kind"] == "scan_train":
             s["dh"] = normal(*lead, D)
             s["dh_last"] = normal(B, D, dtype=torch.float32) if case["carry"] else None
-            s["ckpt"] = None
-            if own:     # the forward pass of the same step, which every training program runs first
-                from triton_snn_fusion_b200.runtime.temporal_gated_scan_backend import run_temporal_gated_scan
-                s["ckpt"] = run_temporal_gated_scan(
-                    s["x"], s["g"], s["h0"], gate=case["gate"], leaky=case["leaky"], lengths=s["lengths"],
-                    batch_first=case["batch_first"], save_for_backward=True).ckpt
     elif case["kind"] in ("norm", "norm_bwd"):
         M, D = case["M"], case["D"]
         s["y"] = normal(M, D, std=2.0)
@@ -196,12 +190,15 @@ def _gates(s):
 
 
 def _states(a, u, h0):
-    h = torch.zeros_like(u[0]) if h0 is None else h0
-    hs = []
-    for at, ut in zip(a.unbind(0), u.unbind(0)):
-        h = at * h + ut
-        hs.append(h)
-    return torch.stack(hs), h
+    """All h_t = a_t h_{t-1} + u_t, time outermost: the span that each step's (product, sum) covers doubles."""
+    if h0 is not None:
+        u = torch.cat([(u[0] + a[0] * h0)[None], u[1:]])
+    span = 1
+    while span < a.shape[0]:
+        u = torch.cat([u[:span], u[span:] + a[span:] * u[:-span]])
+        a = torch.cat([a[:span], a[span:] * a[:-span]])
+        span *= 2
+    return u
 
 
 def _order(case, t, dt):
@@ -211,36 +208,33 @@ def _order(case, t, dt):
 def _scan(s):
     case = s["case"]
     x, a, b, u, live = _gates(s)
-    hs, last = _states(a, u, s["h0"])
+    hs = _states(a, u, s["h0"])
+    last = hs[-1].clone()
     if live is not None:
         hs = torch.where(live, hs, 0.0)
     return _order(case, hs, DTYPES[case["dtype"]]), last
 
 
-def _scan_bwd(s):
+def _scan_train(s):
     case, dt = s["case"], DTYPES[s["case"]["dtype"]]
     x, a, b, u, live = _gates(s)
-    hs, _ = _states(a, u, s["h0"])
+    hs = _states(a, u, s["h0"])
     first = torch.zeros_like(u[0]) if s["h0"] is None else s["h0"]
     before = torch.cat([first[None], hs[:-1]])
     dh = s["dh"].float()
     dh = dh.transpose(0, 1) if case["batch_first"] else dh
     if live is not None:
         dh = torch.where(live, dh, 0.0)
-    lam = torch.zeros_like(first) if s["dh_last"] is None else s["dh_last"]
-    lams = []
-    for t in range(case["T"] - 1, -1, -1):
-        tot = dh[t] + lam
-        lams.append(tot)
-        lam = a[t] * tot
-    lams = torch.stack(lams[::-1])
+    # lam_t = dh_t + a_{t+1} lam_{t+1}: the same recurrence from the end
+    lams = _states(torch.cat([torch.ones_like(first)[None], a.flip(0)[:-1]]), dh.flip(0), s["dh_last"]).flip(0)
     dx = b * lams if case["leaky"] else lams
     dg = lams * (before - x if case["leaky"] else before)
     if case["gate"] == "sigmoid":
         dg = dg * a * b
     if live is not None:
         dx, dg = torch.where(live, dx, 0.0), torch.where(live, dg, 0.0)
-    return _order(case, dx, dt), _order(case, dg, dt), lam
+        hs = torch.where(live, hs, 0.0)
+    return _order(case, hs, dt), _order(case, dx, dt), _order(case, dg, dt), a[0] * lams[0]
 
 
 def _act(kind, gate):
@@ -313,19 +307,19 @@ def _w4(s):
     return y.to(DTYPES[s["case"]["dtype"]])
 
 
-_PLAIN = {"scan": _scan, "scan_bwd": _scan_bwd, "norm": _norm, "norm_bwd": _norm_bwd, "w4": _w4}
+_PLAIN = {"scan": _scan, "scan_train": _scan_train, "norm": _norm, "norm_bwd": _norm_bwd, "w4": _w4}
 
 
 def _own(s):
     case = s["case"]
-    if case["kind"] in ("scan", "scan_bwd"):
+    if case["kind"] in ("scan", "scan_train"):
         from triton_snn_fusion_b200.runtime import temporal_gated_scan_backend as scan
         kw = dict(gate=case["gate"], leaky=case["leaky"], lengths=s["lengths"], batch_first=case["batch_first"])
+        f = scan.run_temporal_gated_scan(s["x"], s["g"], s["h0"], save_for_backward=case["kind"] == "scan_train", **kw)
         if case["kind"] == "scan":
-            r = scan.run_temporal_gated_scan(s["x"], s["g"], s["h0"], **kw)
-            return r.h_seq, r.h_last
-        r = scan.run_temporal_gated_scan_backward(s["dh"], s["x"], s["g"], s["h0"], s["ckpt"], dh_last=s["dh_last"], **kw)
-        return r.dx, r.dgate, r.dh_init
+            return f.h_seq, f.h_last
+        r = scan.run_temporal_gated_scan_backward(s["dh"], s["x"], s["g"], s["h0"], f.ckpt, dh_last=s["dh_last"], **kw)
+        return f.h_seq, r.dx, r.dgate, r.dh_init
     if case["kind"] in ("norm", "norm_bwd"):
         from triton_snn_fusion_b200.runtime import block_norm_backend as norm
         kw = dict(gate=s["gate"], residual=s["r"], w_post=s["w_post"], res_scale=s["scale"], w_pre=s["w_pre"],
@@ -346,13 +340,13 @@ def run(state):
 # -------------------------------------------------------------------------------------------------- work ----
 def work(case):
     sz = SIZE[case["dtype"]]
-    if case["kind"] in ("scan", "scan_bwd"):
+    if case["kind"] in ("scan", "scan_train"):
         T, B, D = case["T"], case["B"], case["D"]
         live, n = sum(_steps(case)) * D, T * B * D
         state = 4 * B * D
         if case["kind"] == "scan":
             return {"bytes": sz * (2 * live + n) + state * (2 if case["carry"] else 1), "flops": 8 * live}
-        return {"bytes": sz * (3 * live + 2 * n) + state * (3 if case["carry"] else 1), "flops": 16 * live}
+        return {"bytes": sz * (3 * live + 3 * n) + state * (3 if case["carry"] else 1), "flops": 24 * live}
     if case["kind"] in ("norm", "norm_bwd"):
         M, D = case["M"], case["D"]
         gate, pre = case["gate"] != "none", case["pre"]
@@ -367,15 +361,13 @@ def work(case):
 
 
 # ----------------------------------------------------------------------------------- 64-bit definitions ----
-def _double_scan(a, u):
-    """All h_t = a_t h_{t-1} + u_t with h_{-1} = 0, by doubling the span of each step's (product, sum)."""
-    a, u = a.clone(), u.clone()
-    span = 1
-    while span < a.shape[0]:
-        u[span:] += a[span:] * u[:-span].clone()
-        a[span:] *= a[:-span].clone()
-        span *= 2
-    return a, u
+def _walk(a, u, h):
+    """h_t = a_t h_{t-1} + u_t step by step."""
+    out = torch.empty_like(u)
+    for t in range(a.shape[0]):
+        h = torch.addcmul(u[t], a[t], h)
+        out[t] = h
+    return out
 
 
 def _exact_scan(case, s, backward):
@@ -390,22 +382,19 @@ def _exact_scan(case, s, backward):
     a = a.masked_fill(pad, 1.0)
     u = u.masked_fill(pad, 0.0)
     h0 = torch.zeros_like(u[0]) if s["h0"] is None else s["h0"].double()
-    prod, h = _double_scan(a, u)
-    h = h + prod * h0
+    h = _walk(a, u, h0)
+    seq = flip(h.masked_fill(pad, 0.0))
     if not backward:
-        last = h[-1]
-        return flip(h.masked_fill(pad, 0.0)), last
+        return seq, h[-1]
     prev = torch.cat((h0[None], h[:-1]))
     dh = flip(s["dh"].double()).masked_fill(pad, 0.0)
-    if s["dh_last"] is not None:
-        dh[-1] += s["dh_last"].double()
-    # the same recurrence from the end: lam_t = a_{t+1} lam_{t+1} + dh_t
-    after = torch.cat((a[1:], torch.zeros_like(a[:1])))
-    lam = _double_scan(after.flip(0), dh.flip(0))[1].flip(0)
+    end = torch.zeros_like(h0) if s["dh_last"] is None else s["dh_last"].double()
+    after = torch.cat((a[1:], torch.ones_like(a[:1])))      # lam_t = a_{t+1} lam_{t+1} + dh_t
+    lam = _walk(after.flip(0), dh.flip(0), end).flip(0)
     dx = (lam * one_less if case["leaky"] else lam).masked_fill(pad, 0.0)
     da = lam * (prev - x if case["leaky"] else prev)
     dg = (da * torch.sigmoid(g) * one_less if case["gate"] == "sigmoid" else da).masked_fill(pad, 0.0)
-    return flip(dx), flip(dg), a[0] * lam[0]
+    return seq, flip(dx), flip(dg), a[0] * lam[0]
 
 
 def _exact_norm(case, s, backward):
@@ -434,14 +423,9 @@ def _exact_norm(case, s, backward):
 
 
 def exact(case, seed):
-    global own
-    was, own = own, False       # the inputs alone
-    try:
-        s = prepare(case, seed)
-    finally:
-        own = was
-    if case["kind"] in ("scan", "scan_bwd"):
-        return _exact_scan(case, s, case["kind"] == "scan_bwd")
+    s = prepare(case, seed)
+    if case["kind"] in ("scan", "scan_train"):
+        return _exact_scan(case, s, case["kind"] == "scan_train")
     if case["kind"] in ("norm", "norm_bwd"):
         return _exact_norm(case, s, case["kind"] == "norm_bwd")
     low, high = s["q"].bitwise_and(15).double(), s["q"].bitwise_right_shift(4).double()
