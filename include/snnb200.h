@@ -57,6 +57,11 @@ extern "C" {
 typedef enum snnb_dtype { SNNB_F32 = 0, SNNB_BF16 = 1, SNNB_F16 = 2, SNNB_U8 = 3, SNNB_B1 = 4 } snnb_dtype;
 typedef enum snnb_layout { SNNB_NCHW = 0, SNNB_NHWC = 1 } snnb_layout;
 
+/* What the gate sequence of snnb_gated_scan holds: the decay itself, or its logit (decay = 1 / (1 + exp(-gate))). */
+typedef enum snnb_gate { SNNB_GATE_VALUE = 0, SNNB_GATE_SIGMOID = 1 } snnb_gate;
+/* Activation of the gate of snnb_block_norm: no gate, sigmoid(g), or g * sigmoid(g). */
+typedef enum snnb_act { SNNB_ACT_NONE = 0, SNNB_ACT_SIGMOID = 1, SNNB_ACT_SILU = 2 } snnb_act;
+
 /* Which conv / linear implementation to use. AUTO picks a tcgen05 kernel when
  * the shape qualifies (16-bit activations, Cin a multiple of 64, see
  * snnb_conv_lif) and the CUDA-core path otherwise. TCGEN05 insists on a tensor-core
@@ -317,6 +322,96 @@ int snnb_maxpool3x3s2_bits(const void *x, void *y, int64_t frames, int H, int W,
 /* out[n][k] = (1/T) sum_t ( fc_w . mean_hw x[t][n] + fc_b ), x NHWC [T][N][HW][C], out fp32. */
 int snnb_avgpool_linear_mean(const void *x_seq, const void *fc_w, const void *fc_b, float *out,
                              int T, int N, int C, int HW, int K, int dtype, void *stream);
+
+/*
+ * Operators of gated recurrent blocks (training and decoding of sequence models on the framework's neurons). No
+ * counterpart in the reference. All arithmetic is fp32 on the widened inputs; every output is rounded once.
+ *
+ * Gated scan: the leaky charge step above without the spike, its leak given per step and channel.
+ *   a_t = gate_t (SNNB_GATE_VALUE) or 1 / (1 + exp(-gate_t)) (SNNB_GATE_SIGMOID)
+ *   h_t = a_t h_{t-1} + (1 - a_t) x_t   if leaky != 0,   h_t = a_t h_{t-1} + x_t   otherwise
+ * for t = 0 .. T-1, each of B sequences and D channels. x, gate, h_seq: rows of D dense values, row (t, b) at
+ * t * _t_stride + b * _b_stride elements, so time or batch may be outermost and rows may be parts of wider ones; the
+ * rows of an output must not overlap.
+ *   h_init [B][D] or NULL (zeros), h_last [B][D] or NULL: state_dtype (the x dtype or SNNB_F32); they may be one
+ *   buffer. No other pair of arguments may overlap.
+ *   lengths [B] (device memory, int32) or NULL: sequence b has lengths[b] steps, clamped to 0 .. T. Later rows of x and
+ *   gate are not read, their rows of h_seq are set to zero, and h_last is the state after the last step that counts.
+ *   ckpt: NULL, or snnb_gated_scan_ckpt_rows(T) * B * D floats (4-byte aligned) that receive the fp32 state before
+ *   every SNNB_GATED_SCAN_CKPT_STEPS-th step for the backward pass. T <= SNNB_GATED_SCAN_CKPT_STEPS needs none.
+ * T = 1 is the step of a decoder; T = 0 copies the state. Gates outside [-1, 1] are taken as they are, but over long
+ * sequences the products of such gates may leave the range of fp32 although every h_t stays inside it.
+ */
+#define SNNB_GATED_SCAN_CKPT_STEPS 128
+int64_t snnb_gated_scan_ckpt_rows(int64_t T);
+int snnb_gated_scan(const void *x, int64_t x_t_stride, int64_t x_b_stride,
+                    const void *gate, int64_t g_t_stride, int64_t g_b_stride,
+                    const void *h_init, const int *lengths,
+                    void *h_seq, int64_t h_t_stride, int64_t h_b_stride, void *h_last, float *ckpt,
+                    int64_t T, int64_t B, int64_t D, int gate_kind, int leaky, int dtype, int state_dtype,
+                    void *stream);
+/*
+ * Gradients of snnb_gated_scan for the gradient dh of h_seq and dh_last of h_last (NULL = zeros):
+ *   lam_t = dh_t + a_{t+1} lam_{t+1};  dx_t = (1 - a_t) lam_t or lam_t;  dh_init = a_0 lam_0;
+ *   dgate_t = lam_t (h_{t-1} - x_t) or lam_t h_{t-1}, times a_t (1 - a_t) for SNNB_GATE_SIGMOID.
+ * x, gate, h_init, lengths as in the forward call, ckpt as it left them. Rows that do not count get zero gradients and
+ * their dh is not read. dh_last and dh_init (may be NULL) have state_dtype and may be one buffer.
+ */
+int snnb_gated_scan_backward(const void *dh, int64_t dh_t_stride, int64_t dh_b_stride, const void *dh_last,
+                             const void *x, int64_t x_t_stride, int64_t x_b_stride,
+                             const void *gate, int64_t g_t_stride, int64_t g_b_stride,
+                             const void *h_init, const float *ckpt, const int *lengths,
+                             void *dx, int64_t dx_t_stride, int64_t dx_b_stride,
+                             void *dgate, int64_t dg_t_stride, int64_t dg_b_stride, void *dh_init,
+                             int64_t T, int64_t B, int64_t D, int gate_kind, int leaky, int dtype, int state_dtype,
+                             void *stream);
+
+/*
+ * The norm behind a block, its gate and residual scale, and the norm in front of the next block, in one pass over M
+ * rows of D values (D <= SNNB_BLOCK_NORM_MAX_D):
+ *   n       = y / sqrt(mean(y^2) + eps) * w_post      (post_norm == 0: n = y, w_post NULL)
+ *   res_out = res + alpha * res_scale * act(gate) * n
+ *   z       = res_out / sqrt(mean(res_out^2) + eps) * w_pre
+ * y NULL: res_out = res and only the norm in front of a block remains (gate, w_post, res_scale NULL, post_norm 0).
+ * res NULL = zeros; gate NULL with SNNB_ACT_NONE; w_post, res_scale, w_pre [D] of w_dtype (the y dtype or SNNB_F32) or
+ * NULL = ones. y, gate, res have rows _stride elements apart; res_out and z are dense [M][D], either may be NULL (z NULL:
+ * no norm in front). res_out may be res itself if its rows are dense; no other pair of arguments may overlap. z is
+ * computed from res_out before its rounding.
+ */
+#define SNNB_BLOCK_NORM_MAX_D 16384
+int snnb_block_norm(const void *y, int64_t y_stride, const void *gate, int64_t gate_stride,
+                    const void *res, int64_t res_stride, const void *w_post, const void *res_scale, const void *w_pre,
+                    void *res_out, void *z, int64_t M, int D, float alpha, float eps, int gate_act, int post_norm,
+                    int dtype, int w_dtype, void *stream);
+/*
+ * Gradients of snnb_block_norm for the gradients dres_out and dz of its results (NULL = zeros; not both). y, gate, res
+ * and the parameters are those of the forward call (res as it was BEFORE an update in place). dy, dgate, dres: dense
+ * [M][D] of the y dtype; dy and dgate are given exactly when y and gate are, dres may be NULL. dw_post, dres_scale,
+ * dw_pre: fp32 [D] or NULL, summed over the rows in a fixed order.
+ * workspace: snnb_block_norm_backward_workspace_bytes(M, D) bytes of device memory, 16-byte aligned, overwritten by the
+ * call; calls that may run at the same time need one each.
+ */
+int64_t snnb_block_norm_backward_workspace_bytes(int64_t M, int D);
+int snnb_block_norm_backward(const void *dres_out, int64_t dres_out_stride, const void *dz, int64_t dz_stride,
+                             const void *y, int64_t y_stride, const void *gate, int64_t gate_stride,
+                             const void *res, int64_t res_stride, const void *w_post, const void *res_scale,
+                             const void *w_pre, void *dy, void *dgate, void *dres,
+                             float *dw_post, float *dres_scale, float *dw_pre,
+                             void *workspace, int64_t workspace_bytes, int64_t M, int D,
+                             float alpha, float eps, int gate_act, int post_norm, int dtype, int w_dtype, void *stream);
+
+/*
+ * Linear layer with 4-bit weights, for the few tokens of a decoding step:
+ *   y[m][n] = sum_k x[m][k] * (q[n][k] - zero[n][k / G]) * scale[n][k / G] + bias[n],   G = group_size
+ *   x [M][K] (rows x_stride elements apart), q_weight [N][K / 2] bytes, 16-byte aligned: weight k in the low (k even) or
+ *   high (k odd) half of byte k / 2; scales [N][ceil(K / G)] and bias [N] (or NULL) in the x dtype; zeros
+ *   [N][ceil(K / G)] uint8, at most 127, or NULL (8 everywhere); y [M][N], rows y_stride elements apart.
+ * K % 32 == 0, G 32, 64 or 128; the last group may be shorter than G. Any M; the weights are read once for every 32
+ * tokens, so beyond a few hundred tokens a 16-bit matrix product over widened weights is the faster way.
+ */
+int snnb_linear_w4(const void *x, int64_t x_stride, const void *q_weight, const void *scales, const void *zeros,
+                   const void *bias, void *y, int64_t y_stride, int64_t M, int K, int N, int group_size, int dtype,
+                   void *stream);
 
 #ifdef __cplusplus
 }

@@ -16,6 +16,8 @@ LIB_PATH = Path(__file__).resolve().parent / "libsnnb200.so"
 SNNB_OK = 0
 F32, BF16, F16, U8, B1 = 0, 1, 2, 3, 4   # B1: spikes packed one bit each along the channel axis
 NCHW, NHWC = 0, 1
+GATE_VALUE, GATE_SIGMOID = 0, 1
+ACT_NONE, ACT_SIGMOID, ACT_SILU = 0, 1, 2
 PATH_AUTO, PATH_SIMT, PATH_TCGEN05, PATH_TCGEN05_TAPS, PATH_TCGEN05_HALO = 0, 1, 2, 3, 4
 
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.uint8: U8}
@@ -62,6 +64,24 @@ SIGNATURES = {
     "snnb_maxpool3x3s2_bits": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "snnb_avgpool_linear_mean": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "snnb_gated_scan_ckpt_rows": (c_int64, [c_int64]),
+    "snnb_gated_scan": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                                c_int, c_int, c_int, c_int, c_void_p]),
+    "snnb_gated_scan_backward": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                                         c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                         c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                         c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "snnb_block_norm": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_void_p, c_int64, c_int, c_float, c_float, c_int, c_int, c_int, c_int,
+                                c_void_p]),
+    "snnb_block_norm_backward_workspace_bytes": (c_int64, [c_int64, c_int]),
+    "snnb_block_norm_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                         c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int,
+                                         c_float, c_float, c_int, c_int, c_int, c_int, c_void_p]),
+    "snnb_linear_w4": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                               c_int64, c_int, c_int, c_int, c_int, c_void_p]),
 }
 
 

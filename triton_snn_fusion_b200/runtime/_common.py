@@ -163,3 +163,26 @@ def stack_frames(xs: Sequence[torch.Tensor]) -> Tuple[torch.Tensor, int, bool]:
 
 def lif_scalars(v_threshold, v_reset, tau):
     return float(v_threshold), float(v_reset), float(tau)
+
+
+def rows_dense(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself if its innermost dimension is dense, else a contiguous copy."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def rows_2d(t: torch.Tensor) -> torch.Tensor:
+    """[..., D] as [rows, D] with dense rows: a view where the strides allow one, else a copy."""
+    t = rows_dense(t)
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
+def launch(symbol: str, device: torch.device, *args) -> None:
+    """Calls a C entry point on the current stream of ``device``, with that device current."""
+    fn = getattr(_lib.lib, symbol)
+    if device.index is None or device.index == torch.cuda.current_device():
+        status = fn(*args, _lib.current_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _lib.current_stream(device))
+    if status != _lib.SNNB_OK:
+        _lib.check(status, symbol)
