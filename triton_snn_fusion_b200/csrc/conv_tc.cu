@@ -437,7 +437,10 @@ extern "C" int snnb_device_status(int *status_out) {
   int h7 = 0;
   const int rc7 = pw_device_status(&h7);
   if (rc7 != SNNB_OK) return rc7;
-  *status_out = h | h2 | h3 | h4 | h5 | h6 | h7;
+  int h8 = 0;
+  const int rc8 = gated_scan_device_status(&h8);
+  if (rc8 != SNNB_OK) return rc8;
+  *status_out = h | h2 | h3 | h4 | h5 | h6 | h7 | h8;
   return SNNB_OK;
 }
 

@@ -12,137 +12,14 @@
 //
 // The backward pass needs h_{t-1} in 32 bits; it recomputes the states of 128 steps at a time from the fp32
 // checkpoints that the forward pass leaves, which is less traffic than reading the 16-bit h and more exact.
-#include "common.cuh"
+//
+// The kernels are in gated_scan_impl.cuh; this file checks the arguments.
+#include "gated_scan.cuh"
 
 namespace snnb {
 namespace {
 
 constexpr int kCkptSteps = SNNB_GATED_SCAN_CKPT_STEPS;
-
-struct Seq {          // rows of D values; element (t, b, d) at t * ts + b * bs + d
-  const void *p;
-  int64_t ts, bs;
-};
-
-struct ScanArgs {
-  Seq x, g, h;        // h: the output of the forward pass, the gradient dh of the backward pass
-  Seq dx, dg;
-  const void *h_init;
-  const void *dh_last;
-  void *h_last;       // forward: last state; backward: dh_init
-  float *ckpt;
-  const int *lengths;
-  int64_t T, B, D;
-  int state_f32;
-};
-
-template <typename T> __device__ __forceinline__ float at(const Seq &s, int64_t t, int64_t b, int64_t d) {
-  return DT<T>::to_f(static_cast<const T *>(s.p)[t * s.ts + b * s.bs + d]);
-}
-template <typename T> __device__ __forceinline__ void put(const Seq &s, int64_t t, int64_t b, int64_t d, float v) {
-  static_cast<T *>(const_cast<void *>(s.p))[t * s.ts + b * s.bs + d] = DT<T>::from_f(v);
-}
-template <typename T> __device__ __forceinline__ float state_at(const void *p, int f32, int64_t i) {
-  if (p == nullptr) return 0.f;
-  return f32 ? static_cast<const float *>(p)[i] : DT<T>::to_f(static_cast<const T *>(p)[i]);
-}
-template <typename T> __device__ __forceinline__ void state_put(void *p, int f32, int64_t i, float v) {
-  if (p == nullptr) return;
-  if (f32) static_cast<float *>(p)[i] = v;
-  else static_cast<T *>(p)[i] = DT<T>::from_f(v);
-}
-
-// Both a and 1 - a keep their relative accuracy: neither is the difference of the other from one.
-template <bool SIG> __device__ __forceinline__ void gate_of(float g, float &a, float &b) {
-  if constexpr (SIG) {
-    const float e = __expf(-fabsf(g));
-    const float big = __fdividef(1.f, 1.f + e), small = e * big;
-    a = g >= 0.f ? big : small;
-    b = g >= 0.f ? small : big;
-  } else {
-    a = g;
-    b = 1.f - g;
-  }
-}
-
-template <typename T, bool SIG, bool LEAKY>
-__global__ void gated_scan_kernel(ScanArgs q) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= q.B * q.D) return;
-  const int64_t b = i / q.D, d = i % q.D;
-  int64_t len = q.T;
-  if (q.lengths) len = min(max((int64_t)q.lengths[b], (int64_t)0), q.T);
-  float h = state_at<T>(q.h_init, q.state_f32, i);
-  for (int64_t t = 0; t < q.T; ++t) {
-    if (t > 0 && t % kCkptSteps == 0 && q.ckpt) q.ckpt[(t / kCkptSteps - 1) * q.B * q.D + i] = h;
-    if (t < len) {
-      float a, bb;
-      gate_of<SIG>(at<T>(q.g, t, b, d), a, bb);
-      const float x = at<T>(q.x, t, b, d);
-      h = fmaf(a, h, LEAKY ? bb * x : x);
-      put<T>(q.h, t, b, d, h);
-    } else {
-      put<T>(q.h, t, b, d, 0.f);
-    }
-  }
-  state_put<T>(q.h_last, q.state_f32, i, h);
-}
-
-template <typename T, bool SIG, bool LEAKY>
-__global__ void gated_scan_backward_kernel(ScanArgs q) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= q.B * q.D) return;
-  const int64_t b = i / q.D, d = i % q.D;
-  int64_t len = q.T;
-  if (q.lengths) len = min(max((int64_t)q.lengths[b], (int64_t)0), q.T);
-  float lam = state_at<T>(q.dh_last, q.state_f32, i);
-  for (int64_t t = len; t < q.T; ++t) {
-    put<T>(q.dx, t, b, d, 0.f);
-    put<T>(q.dg, t, b, d, 0.f);
-  }
-  float before[kCkptSteps];
-  for (int64_t t0 = (len - 1) / kCkptSteps * kCkptSteps; len > 0 && t0 >= 0; t0 -= kCkptSteps) {
-    const int n = (int)min((int64_t)kCkptSteps, len - t0);
-    float h = t0 == 0 ? state_at<T>(q.h_init, q.state_f32, i) : q.ckpt[(t0 / kCkptSteps - 1) * q.B * q.D + i];
-    for (int k = 0; k < n; ++k) {
-      float a, bb;
-      gate_of<SIG>(at<T>(q.g, t0 + k, b, d), a, bb);
-      const float x = at<T>(q.x, t0 + k, b, d);
-      before[k] = h;
-      h = fmaf(a, h, LEAKY ? bb * x : x);
-    }
-    for (int k = n - 1; k >= 0; --k) {
-      float a, bb;
-      gate_of<SIG>(at<T>(q.g, t0 + k, b, d), a, bb);
-      const float x = at<T>(q.x, t0 + k, b, d);
-      lam += at<T>(q.h, t0 + k, b, d);
-      float dg = lam * (LEAKY ? before[k] - x : before[k]);
-      if (SIG) dg *= a * bb;
-      put<T>(q.dx, t0 + k, b, d, LEAKY ? bb * lam : lam);
-      put<T>(q.dg, t0 + k, b, d, dg);
-      lam *= a;
-    }
-  }
-  state_put<T>(q.h_last, q.state_f32, i, lam);
-}
-
-template <typename T, bool BWD>
-void launch(const ScanArgs &q, int gate_kind, int leaky, cudaStream_t s) {
-  const unsigned blocks = (unsigned)((q.B * q.D + 127) / 128);
-  auto go = [&](auto kern) { kern<<<blocks, 128, 0, s>>>(q); };
-  const bool sig = gate_kind == SNNB_GATE_SIGMOID;
-  if constexpr (BWD) {
-    if (sig && leaky) go(gated_scan_backward_kernel<T, true, true>);
-    else if (sig) go(gated_scan_backward_kernel<T, true, false>);
-    else if (leaky) go(gated_scan_backward_kernel<T, false, true>);
-    else go(gated_scan_backward_kernel<T, false, false>);
-  } else {
-    if (sig && leaky) go(gated_scan_kernel<T, true, true>);
-    else if (sig) go(gated_scan_kernel<T, true, false>);
-    else if (leaky) go(gated_scan_kernel<T, false, true>);
-    else go(gated_scan_kernel<T, false, false>);
-  }
-}
 
 // Whether the T * B rows of an output lie apart from one another.
 bool rows_apart(int64_t ts, int64_t bs, int64_t T, int64_t B, int64_t D) {
@@ -159,7 +36,7 @@ bool partly_same(const void *a, const void *b, int64_t bytes) {
 
 int check_common(const ScanArgs &q, int gate_kind, int dtype, int state_dtype, const char *what) {
   SNNB_CHECK_ARG(q.T >= 0 && q.B >= 0 && q.D >= 0, "%s: sizes must not be negative", what);
-  SNNB_CHECK_ARG(q.T <= 0x7fffffffLL && q.B <= 0x7fffffffLL && q.D <= 0x7fffffffLL && q.B * q.D <= (1LL << 36),
+  SNNB_CHECK_ARG(q.T <= (1LL << 30) && q.B <= 0x7fffffffLL && q.D <= 0x7fffffffLL && q.B * q.D <= (1LL << 36),
                  "%s: problem too large", what);
   SNNB_CHECK_ARG(gate_kind == SNNB_GATE_VALUE || gate_kind == SNNB_GATE_SIGMOID, "%s: bad gate kind %d", what, gate_kind);
   SNNB_CHECK_ARG(is_act_dtype(dtype), "%s: unsupported dtype %d", what, dtype);
@@ -170,8 +47,45 @@ int check_common(const ScanArgs &q, int gate_kind, int dtype, int state_dtype, c
   return SNNB_OK;
 }
 
+bool rows16(const ScanSeq &s, int size) {
+  const int n = 16 / size;
+  return s.p == nullptr || (aligned16(s.p) && s.ts % n == 0 && s.bs % n == 0 && s.ts < (1 << 22));      // 128 rows lie within 2^32 bytes
+}
+
+int dispatch(ScanArgs q, bool backward, int gate_kind, int dtype, cudaStream_t s) {
+  // Time outermost and the batch dense inside it: one row of B * D channels.
+  if (q.T <= 1) q.x.ts = q.g.ts = q.h.ts = q.dx.ts = q.dg.ts = 0;      // one step has no use for its time stride
+  auto dense = [&](const ScanSeq &t) { return t.p == nullptr || t.bs == q.D; };
+  if (!q.lengths && q.B > 1 && dense(q.x) && dense(q.g) && dense(q.h) && dense(q.dx) && dense(q.dg)) {
+    q.D *= q.B;
+    q.B = 1;
+  }
+  if (q.B == 1) q.x.bs = q.g.bs = q.h.bs = q.dx.bs = q.dg.bs = 0;
+  const int sz = dtype_size(dtype);
+  auto state16 = [](const void *p) { return aligned16(p); };
+  const bool aligned = q.D % (16 / sz) == 0 && state16(q.h_init) && state16(q.dh_last) && state16(q.h_last) && rows16(q.x, sz) && rows16(q.g, sz) && rows16(q.h, sz) && rows16(q.dx, sz) &&
+                   rows16(q.dg, sz);
+  for (const ScanSeq *t : {&q.x, &q.g, &q.h, &q.dx, &q.dg})
+    if (t->ts >= (1LL << 29))
+      return fail(SNNB_ERR_UNSUPPORTED, "gated_scan: time strides of 2^29 values or more are not implemented");
+  switch (dtype) {
+    case SNNB_F32: return gated_scan_launch<float>(q, backward, gate_kind, aligned, s);
+    case SNNB_BF16: return gated_scan_launch<__nv_bfloat16>(q, backward, gate_kind, aligned, s);
+    default: return gated_scan_launch<__half>(q, backward, gate_kind, aligned, s);
+  }
+}
+
 }  // namespace
 }  // namespace snnb
+
+int snnb::gated_scan_device_status(int *out) {
+  int a = 0, b = 0, c = 0;
+  if (const int rc = gated_scan_status_f32(&a)) return rc;
+  if (const int rc = gated_scan_status_bf16(&b)) return rc;
+  if (const int rc = gated_scan_status_f16(&c)) return rc;
+  *out = a | b | c;
+  return SNNB_OK;
+}
 
 extern "C" int64_t snnb_gated_scan_ckpt_rows(int64_t T) {
   return T <= snnb::kCkptSteps ? 0 : (T - 1) / snnb::kCkptSteps;
@@ -189,20 +103,13 @@ extern "C" int snnb_gated_scan(const void *x, int64_t x_t_stride, int64_t x_b_st
   q.g = {gate, g_t_stride, g_b_stride};
   q.h = {h_seq, h_t_stride, h_b_stride};
   q.h_init = h_init; q.h_last = h_last; q.ckpt = ckpt; q.lengths = lengths;
-  q.T = T; q.B = B; q.D = D; q.state_f32 = state_dtype == SNNB_F32;
+  q.T = T; q.B = B; q.D = D; q.state_f32 = state_dtype == SNNB_F32; q.leaky = leaky != 0;
   if (const int st = check_common(q, gate_kind, dtype, state_dtype, "gated_scan")) return st;
   SNNB_CHECK_ARG(rows_apart(h_t_stride, h_b_stride, T, B, D), "gated_scan: rows of h_seq overlap");
   SNNB_CHECK_ARG(!partly_same(h_init, h_last, B * D * dtype_size(state_dtype)),
                  "gated_scan: h_init and h_last overlap without being the same buffer");
   if (B * D == 0) return SNNB_OK;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case SNNB_F32: launch<float, false>(q, gate_kind, leaky, s); break;
-    case SNNB_BF16: launch<__nv_bfloat16, false>(q, gate_kind, leaky, s); break;
-    default: launch<__half, false>(q, gate_kind, leaky, s); break;
-  }
-  SNNB_CHECK_LAUNCH("gated_scan");
-  return SNNB_OK;
+  return dispatch(q, false, gate_kind, dtype, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int snnb_gated_scan_backward(const void *dh, int64_t dh_t_stride, int64_t dh_b_stride, const void *dh_last,
@@ -221,7 +128,7 @@ extern "C" int snnb_gated_scan_backward(const void *dh, int64_t dh_t_stride, int
   q.dx = {dx, dx_t_stride, dx_b_stride};
   q.dg = {dgate, dg_t_stride, dg_b_stride};
   q.h_init = h_init; q.dh_last = dh_last; q.h_last = dh_init; q.ckpt = const_cast<float *>(ckpt); q.lengths = lengths;
-  q.T = T; q.B = B; q.D = D; q.state_f32 = state_dtype == SNNB_F32;
+  q.T = T; q.B = B; q.D = D; q.state_f32 = state_dtype == SNNB_F32; q.leaky = leaky != 0;
   if (const int st = check_common(q, gate_kind, dtype, state_dtype, "gated_scan_backward")) return st;
   SNNB_CHECK_ARG(T * B * D == 0 || (dx && dgate), "gated_scan_backward: null pointer");
   SNNB_CHECK_ARG(T * B * D == 0 || T <= kCkptSteps || ckpt,
@@ -231,12 +138,5 @@ extern "C" int snnb_gated_scan_backward(const void *dh, int64_t dh_t_stride, int
   SNNB_CHECK_ARG(!partly_same(dh_last, dh_init, B * D * dtype_size(state_dtype)),
                  "gated_scan_backward: dh_last and dh_init overlap without being the same buffer");
   if (B * D == 0) return SNNB_OK;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case SNNB_F32: launch<float, true>(q, gate_kind, leaky, s); break;
-    case SNNB_BF16: launch<__nv_bfloat16, true>(q, gate_kind, leaky, s); break;
-    default: launch<__half, true>(q, gate_kind, leaky, s); break;
-  }
-  SNNB_CHECK_LAUNCH("gated_scan_backward");
-  return SNNB_OK;
+  return dispatch(q, true, gate_kind, dtype, static_cast<cudaStream_t>(stream));
 }
