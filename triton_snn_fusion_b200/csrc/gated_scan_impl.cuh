@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "gated_scan.cuh"
+#include "packed.cuh"
 #include "umma.cuh"
 
 namespace snnb {
@@ -77,74 +78,10 @@ __device__ __forceinline__ void state_store(void *p, int f32, int64_t i, bool ok
   else st_raw<T, N>(static_cast<T *>(p) + i, v);
 }
 
-// Arithmetic on the VEC channels of a thread, two at a time on the packed fp32 pipe (each half rounds like the scalar
-// instruction).
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpair(uint64_t r, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r)); }
-// r = a * b + c
-template <int N>
-__device__ __forceinline__ void v_fma(const float (&a)[N], const float (&b)[N], const float (&c)[N], float (&r)[N]) {
-  if constexpr (N == 1) {
-    r[0] = fmaf(a[0], b[0], c[0]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; k += 2) {
-      uint64_t o;
-      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(o) : "l"(pair(a[k], a[k + 1])), "l"(pair(b[k], b[k + 1])), "l"(pair(c[k], c[k + 1])));
-      unpair(o, r[k], r[k + 1]);
-    }
-  }
-}
-template <int N> __device__ __forceinline__ void v_mul(const float (&a)[N], const float (&b)[N], float (&r)[N]) {
-  if constexpr (N == 1) {
-    r[0] = a[0] * b[0];
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; k += 2) {
-      uint64_t o;
-      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(o) : "l"(pair(a[k], a[k + 1])), "l"(pair(b[k], b[k + 1])));
-      unpair(o, r[k], r[k + 1]);
-    }
-  }
-}
-template <int N> __device__ __forceinline__ void v_add(const float (&a)[N], const float (&b)[N], float (&r)[N]) {
-  if constexpr (N == 1) {
-    r[0] = a[0] + b[0];
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; k += 2) {
-      uint64_t o;
-      asm("add.rn.f32x2 %0, %1, %2;" : "=l"(o) : "l"(pair(a[k], a[k + 1])), "l"(pair(b[k], b[k + 1])));
-      unpair(o, r[k], r[k + 1]);
-    }
-  }
-}
-template <int N> __device__ __forceinline__ void v_set(float (&r)[N], float v) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) r[k] = v;
-}
-
-// a = 1 / (1 + e) and 1 - a = e a with e = exp(-gate): both keep their relative accuracy, neither is the difference of the
-// other from one. Logits below -80 count as -80 (a = 2e-35, no state that fp32 holds beside its input survives that),
-// which keeps e finite and both approximations away from the ends of their range; a NaN stays one.
+// The decay a and 1 - a of each channel.
 template <bool SIG, int N> __device__ __forceinline__ void gates_of(const float (&g)[N], float (&a)[N], float (&b)[N]) {
-  float one[N], t[N], l2[N];
-  v_set(one, 1.f);
   if constexpr (SIG) {
-    v_set(l2, -1.4426950408889634f);
-#pragma unroll
-    for (int k = 0; k < N; ++k) asm("max.NaN.f32 %0, %1, %2;" : "=f"(t[k]) : "f"(g[k]), "f"(-80.f));
-    v_mul(t, l2, t);
-#pragma unroll
-    for (int k = 0; k < N; ++k) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t[k]) : "f"(t[k]));
-    v_add(t, one, a);
-#pragma unroll
-    for (int k = 0; k < N; ++k) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a[k]) : "f"(a[k]));
-    v_mul(t, a, b);
+    v_sigmoid(g, a, b);
   } else {
 #pragma unroll
     for (int k = 0; k < N; ++k) { a[k] = g[k]; b[k] = 1.f - g[k]; }
@@ -174,31 +111,6 @@ template <int SEG, int DIR> __device__ __forceinline__ float join(const float *p
   }
   return v;
 }
-
-template <typename T, int N> __device__ __forceinline__ void widen(const T *p, float (&v)[N]) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = DT<T>::to_f(p[k]);
-}
-
-template <int N> __device__ __forceinline__ void sh_load(const float *p, float (&v)[N]) {
-  const Pack<float, N> r = *reinterpret_cast<const Pack<float, N> *>(p);
-#pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = r.v[k];
-}
-template <int N> __device__ __forceinline__ void sh_store(float *p, const float (&v)[N]) {
-  Pack<float, N> r;
-#pragma unroll
-  for (int k = 0; k < N; ++k) r.v[k] = v[k];
-  *reinterpret_cast<Pack<float, N> *>(p) = r;
-}
-
-// Asynchronous copy of 16 bytes into shared memory past the L1 cache, in which copies on their way would take a whole line
-// each (with copies of 8 bytes through it a third stage made the forward pass half as slow again).
-__device__ __forceinline__ void copy_async16(void *dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(umma::smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 static __device__ int g_scan_status = 0;      // set when a bounded wait gave up
 
