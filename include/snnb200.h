@@ -406,8 +406,8 @@ int snnb_block_norm_backward(const void *dres_out, int64_t dres_out_stride, cons
  *   x [M][K] (rows x_stride elements apart), q_weight [N][K / 2] bytes, 16-byte aligned: weight k in the low (k even) or
  *   high (k odd) half of byte k / 2; scales [N][ceil(K / G)] and bias [N] (or NULL) in the x dtype; zeros
  *   [N][ceil(K / G)] uint8, at most 127, or NULL (8 everywhere); y [M][N], rows y_stride elements apart.
- * K % 32 == 0, G 32, 64 or 128; the last group may be shorter than G. Any M; the weights are read once for every 32
- * tokens, so beyond a few hundred tokens a 16-bit matrix product over widened weights is the faster way.
+ * K % 32 == 0, G 32, 64 or 128; the last group may be shorter than G. N * K < 2^33, M <= 131070. The weights are read
+ * once for every 32 tokens (fp32: 10), so beyond some hundred tokens a product over widened weights is the faster way.
  */
 int snnb_linear_w4(const void *x, int64_t x_stride, const void *q_weight, const void *scales, const void *zeros,
                    const void *bias, void *y, int64_t y_stride, int64_t M, int K, int N, int group_size, int dtype,
