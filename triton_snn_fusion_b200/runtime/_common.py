@@ -176,11 +176,16 @@ def rows_2d(t: torch.Tensor) -> torch.Tensor:
     return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
 
 
+def dense_like(t: torch.Tensor) -> torch.Tensor:
+    """Uninitialised contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def launch(symbol: str, device: torch.device, *args) -> None:
     """Calls a C entry point on the current stream of ``device``, with that device current."""
-    fn = getattr(_lib.lib, symbol)
-    if device.index is None or device.index == torch.cuda.current_device():
-        status = fn(*args, _lib.current_stream(device))
+    fn, index = getattr(_lib.lib, symbol), device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
             status = fn(*args, _lib.current_stream(device))

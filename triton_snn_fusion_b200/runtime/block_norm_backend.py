@@ -16,7 +16,7 @@ from typing import List, NamedTuple, Optional
 import torch
 
 from .. import _lib
-from ._common import Gate, launch, raise_reasons, rows_2d
+from ._common import ACT_DTYPES, Gate, dense_like, launch, raise_reasons, rows_2d
 
 ACTS = {"none": _lib.ACT_NONE, "sigmoid": _lib.ACT_SIGMOID, "silu": _lib.ACT_SILU}
 MAX_D = 16384
@@ -87,6 +87,26 @@ def check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_a
     return g.why
 
 
+def _is_plain(y, rows, params, gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps) -> bool:
+    """Whether nothing needs a second look: what ``check_block_norm_support`` would say yes to, at the price that a decoding
+    step can pay. Anything else goes through the full check."""
+    if not (type(y) is torch.Tensor and y.is_cuda and y.dim() >= 1 and y.dtype in ACT_DTYPES and eps >= 0.0
+            and (gate is None) == (gate_act == "none") and gate_act in ACTS
+            and (post_norm or w_post is None) and (pre_norm or w_pre is None)):
+        return False
+    shape, dtype, device = y.shape, y.dtype, y.device
+    D = shape[-1]
+    if not 1 <= D <= MAX_D:
+        return False
+    for t in rows:
+        if t is not None and not (type(t) is torch.Tensor and t.shape == shape and t.dtype == dtype and t.device == device):
+            return False
+    for w in params:
+        if w is not None and not (type(w) is torch.Tensor and w.shape == (D,) and w.dtype == dtype and w.device == device):
+            return False
+    return True
+
+
 def _params(lead, *ws):
     ws = [w.contiguous() if w is not None else None for w in ws]
     dtype = next((w.dtype for w in ws if w is not None), lead.dtype)
@@ -97,7 +117,7 @@ def _rows(t):
     """[..., D] -> (rows tensor kept alive, address, row stride)."""
     if t is None:
         return None, None, 0
-    r = rows_2d(t)
+    r = t if t.dim() == 2 and t.stride(1) == 1 else rows_2d(t)
     return r, r.data_ptr(), r.stride(0)
 
 
@@ -123,8 +143,9 @@ def run_block_norm(
     ``w_post``, ``res_scale`` and ``w_pre`` may be None (zeros, ones, ones, ones); the parameters are [D] in y's dtype or
     fp32. ``res_inplace`` writes res_out over ``residual``, which must be contiguous then.
     """
-    raise_reasons("block_norm", check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm,
-                                                         pre_norm, eps), False, verbose)
+    if not _is_plain(y, (gate, residual), (w_post, res_scale, w_pre), gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps):
+        raise_reasons("block_norm", check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm,
+                                                             pre_norm, eps), False, verbose)
     lead = y if y is not None else residual
     if y is None and not pre_norm:
         raise RuntimeError("unsupported_form: neither y nor pre_norm, nothing to compute")
@@ -134,8 +155,8 @@ def run_block_norm(
     M = lead.numel() // D
     res_out = None
     if y is not None:
-        res_out = residual if res_inplace else torch.empty(lead.shape, dtype=lead.dtype, device=lead.device)
-    z = torch.empty(lead.shape, dtype=lead.dtype, device=lead.device) if pre_norm else None
+        res_out = residual if res_inplace else dense_like(lead)
+    z = dense_like(lead) if pre_norm else None
     (w_post, res_scale, w_pre), w_code = _params(lead, w_post, res_scale, w_pre)
     if M > 0:
         y2, yp, ys = _rows(y)
@@ -170,29 +191,24 @@ def run_block_norm_backward(
     dy, dgate and dresidual are dense in y's dtype; the parameters' gradients are fp32, summed over the rows in a fixed
     order, and None for a parameter that is None.
     """
-    why = check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm, pre_norm, eps,
-                                   dres_out=dres_out, dz=dz)
-    if dres_out is None and dz is None:
-        why.append("unsupported_form: neither dres_out nor dz")
-    if dz is not None and not pre_norm:
-        why.append("unsupported_form: dz is given although pre_norm is off")
-    raise_reasons("block_norm_backward", why, False, verbose)
+    if (dres_out is None and dz is None) or (dz is not None and not pre_norm) or not _is_plain(
+            y, (gate, residual, dres_out, dz), (w_post, res_scale, w_pre), gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps):
+        why = check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm, pre_norm, eps,
+                                       dres_out=dres_out, dz=dz)
+        if dres_out is None and dz is None:
+            why.append("unsupported_form: neither dres_out nor dz")
+        if dz is not None and not pre_norm:
+            why.append("unsupported_form: dz is given although pre_norm is off")
+        raise_reasons("block_norm_backward", why, False, verbose)
     lead = y if y is not None else residual
     D = int(lead.shape[-1])
     M = lead.numel() // D
 
-    def rows_out(have=True):
-        return torch.empty(lead.shape, dtype=lead.dtype, device=lead.device) if have else None
-
-    def sums_out(w):
-        if w is None:
-            return None
-        # without rows, or without a gradient of z, the sum is empty
-        make = torch.zeros if M == 0 or (w is w_pre and dz is None) else torch.empty
-        return make((D,), dtype=torch.float32, device=lead.device)
-
-    dy, dgate, dres = rows_out(y is not None), rows_out(gate is not None), rows_out()
-    dw_post, dscale, dw_pre = sums_out(w_post), sums_out(res_scale), sums_out(w_pre)
+    dy, dgate = dense_like(lead) if y is not None else None, dense_like(lead) if gate is not None else None
+    dres = dense_like(lead)
+    # without rows, or without a gradient of z, a sum is empty
+    sums = (torch.empty if M > 0 and dz is not None else torch.zeros)((3, D), dtype=torch.float32, device=lead.device).unbind(0)
+    dw_post, dscale, dw_pre = (s if w is not None else None for s, w in zip(sums, (w_post, res_scale, w_pre)))
     if M > 0:
         (wp, sc, wr), w_code = _params(lead, w_post, res_scale, w_pre)
         ws = torch.empty(_lib.lib.snnb_block_norm_backward_workspace_bytes(M, D), dtype=torch.uint8, device=lead.device)

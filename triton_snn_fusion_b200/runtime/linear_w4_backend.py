@@ -13,7 +13,7 @@ from typing import List, NamedTuple, Optional
 import torch
 
 from .. import _lib
-from ._common import Gate, launch, raise_reasons, rows_2d
+from ._common import ACT_DTYPES, Gate, launch, raise_reasons, rows_2d
 
 GROUP_SIZES = (32, 64, 128)
 
@@ -91,6 +91,22 @@ def check_linear_w4_support(x, q_weight, scales, zeros, bias, group_size) -> Lis
     return g.why
 
 
+def _is_plain(x, q, s, z, b, group_size) -> bool:
+    """Whether nothing needs a second look: what ``check_linear_w4_support`` would say yes to, at the price that a decoding
+    step can pay. Anything else goes through the full check."""
+    if not (type(x) is torch.Tensor and type(q) is torch.Tensor and type(s) is torch.Tensor and x.is_cuda and x.dim() >= 1
+            and q.dim() == 2 and x.dtype in ACT_DTYPES and group_size in GROUP_SIZES):
+        return False
+    K, (N, half), dtype, device = x.shape[-1], q.shape, x.dtype, x.device
+    if not (K > 0 and K % 32 == 0 and 2 * half == K and N > 0 and q.dtype == torch.uint8 and s.dtype == dtype
+            and q.device == device and s.device == device):
+        return False
+    groups = (N, -(-K // group_size))
+    return (s.shape == groups
+            and (z is None or (type(z) is torch.Tensor and z.shape == groups and z.dtype == torch.uint8 and z.device == device))
+            and (b is None or (type(b) is torch.Tensor and b.shape == (N,) and b.dtype == dtype and b.device == device)))
+
+
 def run_linear_w4(
     x: torch.Tensor,
     q_weight: torch.Tensor,
@@ -104,7 +120,8 @@ def run_linear_w4(
 ) -> torch.Tensor:
     """x [..., K] -> [..., N] in x's dtype. ``q_weight``, ``scales`` and ``zeros`` as ``quantize_linear_w4`` lays them out;
     keep them contiguous (they are copied at every call otherwise). ``out``: a contiguous tensor to write into."""
-    raise_reasons("linear_w4", check_linear_w4_support(x, q_weight, scales, zeros, bias, group_size), False, verbose)
+    if not _is_plain(x, q_weight, scales, zeros, bias, group_size):
+        raise_reasons("linear_w4", check_linear_w4_support(x, q_weight, scales, zeros, bias, group_size), False, verbose)
     K, N = int(x.shape[-1]), int(q_weight.shape[0])
     shape = (*x.shape[:-1], N)
     if out is None:

@@ -17,7 +17,7 @@ from typing import List, NamedTuple, Optional
 import torch
 
 from .. import _lib
-from ._common import Gate, launch, raise_reasons, rows_dense, state_or_none
+from ._common import ACT_DTYPES, Gate, dense_like, launch, raise_reasons, rows_dense, state_or_none
 
 GATES = {"value": _lib.GATE_VALUE, "sigmoid": _lib.GATE_SIGMOID}
 
@@ -72,6 +72,16 @@ def check_temporal_gated_scan_support(x_seq, gate_seq, h_init, gate, lengths=Non
     return g.why
 
 
+def _is_plain(x, g, gate, h0, lengths, batch_first, state_dtype) -> bool:
+    """Whether nothing needs a second look: what ``check_temporal_gated_scan_support`` would say yes to, at the price that a
+    decoding step can pay. Anything else goes through the full check."""
+    return (type(x) is torch.Tensor and type(g) is torch.Tensor and x.is_cuda and x.dim() == 3 and x.dtype in ACT_DTYPES
+            and g.shape == x.shape and g.dtype == x.dtype and g.device == x.device and gate in GATES
+            and (h0 is None or (type(h0) is torch.Tensor and h0.dtype == torch.float32 and h0.device == x.device
+                                and h0.shape == (x.shape[0 if batch_first else 1], x.shape[2])))
+            and lengths is None and state_dtype is None)
+
+
 def _strides(t, batch_first):
     s = t.stride()
     return (s[1], s[0]) if batch_first else (s[0], s[1])
@@ -109,9 +119,10 @@ def run_temporal_gated_scan(
     ``h_last_out`` may be ``h_init`` itself (a decoder's state updated in place). Rows may be parts of wider ones (x and
     gate as two halves of one projection); an innermost dimension that is not dense is copied first.
     """
-    raise_reasons("temporal_gated_scan",
-                  check_temporal_gated_scan_support(x_seq, gate_seq, h_init, gate, lengths, batch_first, state_dtype),
-                  False, verbose)
+    if not _is_plain(x_seq, gate_seq, gate, h_init, lengths, batch_first, state_dtype):
+        raise_reasons("temporal_gated_scan",
+                      check_temporal_gated_scan_support(x_seq, gate_seq, h_init, gate, lengths, batch_first, state_dtype),
+                      False, verbose)
     T, B, D = _sizes(x_seq, batch_first)
     x, g = rows_dense(x_seq), rows_dense(gate_seq)
     h0 = state_or_none(h_init)
@@ -119,7 +130,7 @@ def run_temporal_gated_scan(
     h0 = h0.contiguous() if h0 is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
     if h_seq_out is None:
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = dense_like(x)
     else:
         h = h_seq_out
         if h.shape != x.shape or h.dtype != x.dtype or h.device != x.device or (D > 1 and h.stride(2) != 1):
@@ -177,8 +188,7 @@ def run_temporal_gated_scan_backward(
     h0 = h0.contiguous() if h0 is not None else None
     dl = dl.contiguous() if dl is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dg = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx, dg = dense_like(x), dense_like(x)
     dh_init = torch.empty((B, D), dtype=s_dt, device=x.device)
     launch("snnb_gated_scan_backward", x.device,
            dh.data_ptr(), *_strides(dh, batch_first), _lib.ptr(dl), x.data_ptr(), *_strides(x, batch_first),
