@@ -339,7 +339,8 @@ int snnb_avgpool_linear_mean(const void *x_seq, const void *fc_w, const void *fc
  *   gate are not read, their rows of h_seq are set to zero, and h_last is the state after the last step that counts.
  *   ckpt: NULL, or snnb_gated_scan_ckpt_rows(T) * B * D floats (4-byte aligned) that receive the fp32 state before
  *   every SNNB_GATED_SCAN_CKPT_STEPS-th step for the backward pass. T <= SNNB_GATED_SCAN_CKPT_STEPS needs none.
- * T = 1 is the step of a decoder; T = 0 copies the state. Gates outside [-1, 1] are taken as they are, but over long
+ * T = 1 is the step of a decoder; T = 0 copies the state. T <= 2^30, B * D <= 2^36, and for T > 1 a _t_stride is below
+ * 2^29 (SNNB_ERR_UNSUPPORTED otherwise). Gates outside [-1, 1] are taken as they are, but over long
  * sequences the products of such gates may leave the range of fp32 although every h_t stays inside it.
  */
 #define SNNB_GATED_SCAN_CKPT_STEPS 128
@@ -355,7 +356,8 @@ int snnb_gated_scan(const void *x, int64_t x_t_stride, int64_t x_b_stride,
  *   lam_t = dh_t + a_{t+1} lam_{t+1};  dx_t = (1 - a_t) lam_t or lam_t;  dh_init = a_0 lam_0;
  *   dgate_t = lam_t (h_{t-1} - x_t) or lam_t h_{t-1}, times a_t (1 - a_t) for SNNB_GATE_SIGMOID.
  * x, gate, h_init, lengths as in the forward call, ckpt as it left them. Rows that do not count get zero gradients and
- * their dh is not read. dh_last and dh_init (may be NULL) have state_dtype and may be one buffer.
+ * their dh is not read. dh_last and dh_init (may be NULL) have state_dtype and may be one buffer; no other pair of
+ * arguments of which one is written may overlap.
  */
 int snnb_gated_scan_backward(const void *dh, int64_t dh_t_stride, int64_t dh_b_stride, const void *dh_last,
                              const void *x, int64_t x_t_stride, int64_t x_b_stride,
@@ -387,7 +389,7 @@ int snnb_block_norm(const void *y, int64_t y_stride, const void *gate, int64_t g
  * Gradients of snnb_block_norm for the gradients dres_out and dz of its results (NULL = zeros; not both). y, gate, res
  * and the parameters are those of the forward call (res as it was BEFORE an update in place). dy, dgate, dres: dense
  * [M][D] of the y dtype; dy and dgate are given exactly when y and gate are, dres may be NULL. dw_post, dres_scale,
- * dw_pre: fp32 [D] or NULL, summed over the rows in a fixed order.
+ * dw_pre: fp32 [D] or NULL, summed over the rows in a fixed order. No output overlaps an input or another output.
  * workspace: snnb_block_norm_backward_workspace_bytes(M, D) bytes of device memory, 16-byte aligned, overwritten by the
  * call; calls that may run at the same time need one each.
  */
@@ -405,7 +407,8 @@ int snnb_block_norm_backward(const void *dres_out, int64_t dres_out_stride, cons
  *   y[m][n] = sum_k x[m][k] * (q[n][k] - zero[n][k / G]) * scale[n][k / G] + bias[n],   G = group_size
  *   x [M][K] (rows x_stride elements apart), q_weight [N][K / 2] bytes, 16-byte aligned: weight k in the low (k even) or
  *   high (k odd) half of byte k / 2; scales [N][ceil(K / G)] and bias [N] (or NULL) in the x dtype; zeros
- *   [N][ceil(K / G)] uint8, at most 127, or NULL (8 everywhere); y [M][N], rows y_stride elements apart.
+ *   [N][ceil(K / G)] uint8, at most 127, or NULL (8 everywhere); y [M][N], rows y_stride elements apart,
+ *   apart from x.
  * K % 32 == 0, G 32, 64 or 128; the last group may be shorter than G. N * K < 2^33, M <= 131070. The weights are read
  * once for every 32 tokens (fp32: 10), so beyond some hundred tokens a product over widened weights is the faster way.
  */

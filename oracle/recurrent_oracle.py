@@ -3,8 +3,9 @@
 Each function returns its results and, for every value, a bound on the absolute error of an evaluation in fp32 whose
 roundings are counted in units of 2^-24: the formula evaluated on magnitudes times that count. The counts:
 
-  sigmoid   __expf is off by at most 2 + 1.173 |g| units of 2^-23, the reciprocal by 2, the sum by 1/2: for |g| <= 8
-            under 32 units of 2^-24, for a gate and for one minus it alike (each is formed without a difference)
+  sigmoid   e = 2^(-g log2 e): the product's rounding and the constant's make at most 2 |g| units, the approximate power
+            of two 4, the sum 1, the approximate reciprocal 2 and the product with e 1: for |g| <= 8 under 32 units of
+            2^-24, for a gate and for one minus it alike (each is formed without a difference)
   scan      a step adds a product, a sum and (where parts of a sequence are joined) one factor of a product of gates:
             40 units of the magnitude, which is the recurrence of |u| (parts may cancel), carried on by the recurrence
   norm      a sum of D squares in 256 or more lanes: D / 256 + 10 <= 74 units, halved by the root, the root 4, the

@@ -219,6 +219,28 @@ def test_results_repeat_and_graphs_do_not_share_a_workspace():
 
 
 @gpu
+def test_more_than_2_to_32_bytes():
+    """One row repeated 132000 times (4.3 GB a result): each row comes out as the first; the parameters' gradients are that
+    row's times the number of rows, to within a rounding a row added in fp32 (at most 132040 units of 2^-24)."""
+    M, D = 132000, 16384
+    v, dro, dz = _inputs(1, D, torch.bfloat16)
+    dv = {k: _dev(t) for k, t in v.items()}
+    rows = lambda t: _dev(t).expand(M, D)  # noqa: E731
+    w = dict(w_post=dv["w_post"], res_scale=dv["res_scale"], w_pre=dv["w_pre"], gate_act="silu")
+    one = ops.run_block_norm(dv["y"], gate=dv["gate"], residual=dv["residual"], **w)
+    f = ops.run_block_norm(rows(v["y"]), gate=rows(v["gate"]), residual=rows(v["residual"]), **w)
+    for m in (0, M // 2, M - 1):
+        assert torch.equal(f.z[m], one.z[0]) and torch.equal(f.res_out[m], one.res_out[0])
+    del f
+    one = ops.run_block_norm_backward(_dev(dro), _dev(dz), dv["y"], gate=dv["gate"], residual=dv["residual"], **w)
+    r = ops.run_block_norm_backward(rows(dro), rows(dz), rows(v["y"]), gate=rows(v["gate"]), residual=rows(v["residual"]), **w)
+    for m in (0, M // 2, M - 1):
+        assert torch.equal(r.dy[m], one.dy[0]) and torch.equal(r.dgate[m], one.dgate[0]) and torch.equal(r.dresidual[m], one.dresidual[0])
+    for a, b in zip(r[3:], one[3:]):
+        assert bool(((a.double() - M * b.double()).abs() <= (M + 40) * 2.0 ** -24 * M * b.double().abs()).all())
+
+
+@gpu
 def test_gradients_against_differences():
     """Central differences of the forward pass for J = sum(dres_out * res_out) + sum(dz * z): step 2^-6, fp32."""
     v, dro, dz = _inputs(7, 64, torch.float32)
@@ -253,7 +275,8 @@ def test_c_refusals():
                            (dict(act=0), 1, "gate"), (dict(g=None), 1, "gate"), (dict(act=3), 1, "activation"),
                            (dict(dt=3), 1, "dtype"), (dict(wdt=2), 1, "parameter dtype"), (dict(eps=-1.0), 1, "eps"),
                            (dict(y=None), 1, "belong to y"), (dict(post=0), 1, "w_post"), (dict(ro=None, z=None), 1, "neither"),
-                           (dict(z=None), 1, "w_pre"), (dict(ro=12288, rs=128), 1, "in place"), (dict(gs=-1), 1, "stride")):
+                           (dict(z=None), 1, "w_pre"), (dict(ro=12288, rs=128), 1, "in place"), (dict(gs=-1), 1, "stride"), (dict(z=28672), 1, "z shares"), (dict(z=12288), 1, "z shares"),
+                           (dict(ro=4096), 1, "res_out shares")):
         st, msg = _c("snnb_block_norm", base, **kw)
         assert st == code and text in msg, (kw, st, msg)
 
@@ -264,7 +287,7 @@ def test_c_backward_refusals():
                 alpha=1.0, eps=1e-6, act=2, post=1, dt=1, wdt=1, stream=None)
     for kw, text in ((dict(dro=None, dz=None), "neither"), (dict(dz=None), "w_pre without dz"), (dict(dy=None), "dy belongs"),
                      (dict(dg=None), "dgate belongs"), (dict(wb=16), "workspace too small"), (dict(ws=None), "workspace"),
-                     (dict(ws=65540), "aligned")):
+                     (dict(ws=65540), "aligned"), (dict(dy=12288), "one of the inputs"), (dict(dg=45056), "one buffer")):
         st, msg = _c("snnb_block_norm_backward", base, **kw)
         assert st == 1 and text in msg, (kw, st, msg)
 

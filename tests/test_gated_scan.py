@@ -241,6 +241,27 @@ def test_results_repeat_bit_for_bit_and_in_a_graph_on_another_stream():
 
 
 @gpu
+def test_more_than_2_to_32_bytes():
+    """A constant input and gate, never stored more than once: every state is x (1 - a^(t+1)), which is x in bf16 from step
+    100 on (a <= 0.9, 0.9^100 < 2^-15). h takes 4.3 GB."""
+    T, D = 33000, 65536
+    x = torch.randn(1, 1, D, generator=torch.Generator().manual_seed(0)).to(DEV).bfloat16()
+    gate = (torch.rand(1, 1, D, generator=torch.Generator().manual_seed(1)) * 4 - 2).to(DEV).bfloat16()
+    h = ops.run_temporal_gated_scan(x.expand(T, 1, D), gate.expand(T, 1, D)).h_seq
+    for t in (200, T // 2, T - 129, T - 1):
+        orc.assert_within(h[t], x[0].double(), x[0].double().abs() * 2.0 ** -12)
+    del h
+    # the same where a row is more than 2^22 values apart from the next
+    wide = torch.empty(40, 1 << 23, dtype=torch.bfloat16, device=DEV)
+    xs, gs, h0, *_ = _inputs(40, 1, 64, torch.bfloat16, "sigmoid")
+    wide[:, :64].copy_(xs[:, 0])
+    wide[:, 1 << 22:(1 << 22) + 64].copy_(gs[:, 0])
+    f = ops.run_temporal_gated_scan(wide[:, None, :64], wide[:, None, 1 << 22:(1 << 22) + 64], h0.to(DEV))
+    want, err, *_ = orc.gated_scan(xs, gs, h0, "sigmoid", True)
+    orc.assert_within(f.h_seq, want, err)
+
+
+@gpu
 def test_gradients_against_differences():
     """Central differences of the kernel's own forward pass in a random direction, for the value
     J = sum(dh * h) + sum(dh_last * h_last). With a step e the difference has the truncation error
@@ -286,7 +307,9 @@ def test_c_refusals():
     for kw, text in ((dict(x=None), "null pointer"), (dict(g=None), "null pointer"), (dict(h=None), "null pointer"),
                      (dict(T=-1), "negative"), (dict(kind=2), "gate kind"), (dict(dt=3), "dtype"), (dict(sdt=2), "state dtype"),
                      (dict(xt=-64), "negative stride"), (dict(ht=32), "overlap"), (dict(B=2, hb=64, ht=64), "overlap"),
-                     (dict(h0=65536, hl=65536 + 16), "overlap"), (dict(T=1 << 40), "too large")):
+                     (dict(h0=65536, hl=65536 + 16), "overlap"), (dict(T=1 << 40), "too large"),
+                     (dict(h=4096), "one of the inputs"), (dict(h=8192), "one of the inputs"),
+                     (dict(T=1 << 30, B=1 << 18, D=1 << 18, hb=1 << 18, ht=1 << 36, x=None), "null pointer")):
         status, msg = _c_call(**kw)
         assert status == 1 and text in msg, (kw, status, msg)
 
@@ -296,7 +319,8 @@ def test_c_backward_refusals():
                 dx=16384, dxt=64, dxb=64, dg=20480, dgt=64, dgb=64, di=None, T=129, B=1, D=64, kind=1, leaky=1, dt=1,
                 sdt=0, stream=None)
     for kw, text in ((dict(), "checkpoints"), (dict(T=2, dx=None), "null pointer"), (dict(T=2, dxt=8), "overlap"),
-                     (dict(T=2, dl=65536, di=65540), "overlap")):
+                     (dict(T=2, dl=65536, di=65540), "overlap"), (dict(T=2, dx=4096), "one of the inputs"),
+                     (dict(T=2, dg=16384), "one buffer")):
         a = dict(base, **kw)
         assert _lib.lib.snnb_gated_scan_backward(*a.values()) == 1
         assert text in _lib.lib.snnb_last_error().decode(), kw

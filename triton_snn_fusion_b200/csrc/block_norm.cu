@@ -882,6 +882,10 @@ extern "C" int snnb_block_norm(const void *y, int64_t y_stride, const void *gate
   SNNB_CHECK_ARG(!res || res_out != res || M <= 1 || res_stride == D,
                  "block_norm: res can be updated in place only if its rows are dense");
   if (M == 0) return SNNB_OK;
+  for (const void *in : {y, gate, (const void *)res_out})
+    SNNB_CHECK_ARG(!z || z != in, "block_norm: z shares its buffer with another argument");
+  SNNB_CHECK_ARG(!z || z != res, "block_norm: z shares its buffer with another argument");
+  SNNB_CHECK_ARG(!res_out || (res_out != y && res_out != gate), "block_norm: res_out shares its buffer with y or the gate");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case SNNB_F32: launch_forward<float>(q, dtype, s); break;
@@ -921,6 +925,12 @@ extern "C" int snnb_block_norm_backward(const void *dres_out, int64_t dres_out_s
   SNNB_CHECK_ARG(!dw_post || post_norm, "block_norm_backward: dw_post without the norm it belongs to");
   SNNB_CHECK_ARG(!dres_scale || y || M == 0, "block_norm_backward: dres_scale without y");
   SNNB_CHECK_ARG(!dw_pre || dz || M == 0, "block_norm_backward: dw_pre without dz");
+  const void *outs[] = {dy, dgate, dres}, *ins[] = {dres_out, dz, y, gate, res};
+  for (int i = 0; i < 3; ++i) {
+    for (const void *in : ins)
+      SNNB_CHECK_ARG(!outs[i] || outs[i] != in, "block_norm_backward: an output is one of the inputs");
+    SNNB_CHECK_ARG(!outs[i] || outs[i] != outs[(i + 1) % 3], "block_norm_backward: two outputs are one buffer");
+  }
   SNNB_CHECK_ARG(workspace && workspace_bytes >= snnb_block_norm_backward_workspace_bytes(M, D),
                  "block_norm_backward: workspace too small");
   SNNB_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "block_norm_backward: workspace must be 16-byte aligned");

@@ -34,6 +34,8 @@ bool partly_same(const void *a, const void *b, int64_t bytes) {
   return p && q && p != q && p < q + (uintptr_t)bytes && q < p + (uintptr_t)bytes;
 }
 
+bool some(int64_t T, int64_t B, int64_t D) { return T > 0 && B > 0 && D > 0; }
+
 int check_common(const ScanArgs &q, int gate_kind, int dtype, int state_dtype, const char *what) {
   SNNB_CHECK_ARG(q.T >= 0 && q.B >= 0 && q.D >= 0, "%s: sizes must not be negative", what);
   SNNB_CHECK_ARG(q.T <= (1LL << 30) && q.B <= 0x7fffffffLL && q.D <= 0x7fffffffLL && q.B * q.D <= (1LL << 36),
@@ -43,7 +45,7 @@ int check_common(const ScanArgs &q, int gate_kind, int dtype, int state_dtype, c
   SNNB_CHECK_ARG(state_dtype == dtype || state_dtype == SNNB_F32, "%s: state dtype must be the x dtype or f32", what);
   SNNB_CHECK_ARG(q.x.ts >= 0 && q.x.bs >= 0 && q.g.ts >= 0 && q.g.bs >= 0 && q.h.ts >= 0 && q.h.bs >= 0,
                  "%s: negative stride", what);
-  if (q.T * q.B * q.D > 0) SNNB_CHECK_ARG(q.x.p && q.g.p && q.h.p, "%s: null pointer", what);
+  if (some(q.T, q.B, q.D)) SNNB_CHECK_ARG(q.x.p && q.g.p && q.h.p, "%s: null pointer", what);
   return SNNB_OK;
 }
 
@@ -105,6 +107,7 @@ extern "C" int snnb_gated_scan(const void *x, int64_t x_t_stride, int64_t x_b_st
   q.h_init = h_init; q.h_last = h_last; q.ckpt = ckpt; q.lengths = lengths;
   q.T = T; q.B = B; q.D = D; q.state_f32 = state_dtype == SNNB_F32; q.leaky = leaky != 0;
   if (const int st = check_common(q, gate_kind, dtype, state_dtype, "gated_scan")) return st;
+  SNNB_CHECK_ARG(!h_seq || (h_seq != x && h_seq != gate), "gated_scan: h_seq is one of the inputs");
   SNNB_CHECK_ARG(rows_apart(h_t_stride, h_b_stride, T, B, D), "gated_scan: rows of h_seq overlap");
   SNNB_CHECK_ARG(!partly_same(h_init, h_last, B * D * dtype_size(state_dtype)),
                  "gated_scan: h_init and h_last overlap without being the same buffer");
@@ -130,8 +133,11 @@ extern "C" int snnb_gated_scan_backward(const void *dh, int64_t dh_t_stride, int
   q.h_init = h_init; q.dh_last = dh_last; q.h_last = dh_init; q.ckpt = const_cast<float *>(ckpt); q.lengths = lengths;
   q.T = T; q.B = B; q.D = D; q.state_f32 = state_dtype == SNNB_F32; q.leaky = leaky != 0;
   if (const int st = check_common(q, gate_kind, dtype, state_dtype, "gated_scan_backward")) return st;
-  SNNB_CHECK_ARG(T * B * D == 0 || (dx && dgate), "gated_scan_backward: null pointer");
-  SNNB_CHECK_ARG(T * B * D == 0 || T <= kCkptSteps || ckpt,
+  SNNB_CHECK_ARG(!some(T, B, D) || (dx && dgate), "gated_scan_backward: null pointer");
+  for (const void *out : {(const void *)dx, (const void *)dgate})
+    SNNB_CHECK_ARG(!out || (out != dh && out != x && out != gate), "gated_scan_backward: an output is one of the inputs");
+  SNNB_CHECK_ARG(!dx || dx != dgate, "gated_scan_backward: dx and dgate are one buffer");
+  SNNB_CHECK_ARG(!some(T, B, D) || T <= kCkptSteps || ckpt,
                  "gated_scan_backward: more than %d steps need the checkpoints of the forward pass", kCkptSteps);
   SNNB_CHECK_ARG(rows_apart(dx_t_stride, dx_b_stride, T, B, D) && rows_apart(dg_t_stride, dg_b_stride, T, B, D),
                  "gated_scan_backward: rows of dx or dgate overlap");

@@ -397,6 +397,7 @@ extern "C" int snnb_linear_w4(const void *x, int64_t x_stride, const void *q_wei
   if (M == 0) return SNNB_OK;
   SNNB_CHECK_ARG(x && q_weight && scales && y, "linear_w4: null pointer");
   SNNB_CHECK_ARG(x_stride >= 0 && (M <= 1 || y_stride >= N), "linear_w4: bad row stride");
+  SNNB_CHECK_ARG(y != x, "linear_w4: y is x");
   SNNB_CHECK_ARG(aligned16(q_weight), "linear_w4: q_weight must be 16-byte aligned");
   W4Args a;
   a.x = x; a.scales = scales; a.bias = bias; a.q = static_cast<const uint8_t *>(q_weight);

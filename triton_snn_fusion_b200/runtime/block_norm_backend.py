@@ -141,7 +141,8 @@ def run_block_norm(
 
     ``y=None`` (with ``post_norm=False``) is the norm in front of the first block: z alone, res_out is None. ``residual``,
     ``w_post``, ``res_scale`` and ``w_pre`` may be None (zeros, ones, ones, ones); the parameters are [D] in y's dtype or
-    fp32. ``res_inplace`` writes res_out over ``residual``, which must be contiguous then.
+    fp32. ``res_inplace`` writes res_out over ``residual``, which must be contiguous and share no
+    memory with y or gate then.
     """
     if not _is_plain(y, (gate, residual), (w_post, res_scale, w_pre), gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps):
         raise_reasons("block_norm", check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm,

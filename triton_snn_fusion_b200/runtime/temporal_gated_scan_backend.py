@@ -116,7 +116,8 @@ def run_temporal_gated_scan(
     ``h_init``: state to start from, None or a 0-dim tensor for zeros. The state is fp32 unless ``h_init`` or
     ``state_dtype`` says it has x_seq's dtype. ``lengths`` (int32 [B], on the device): steps of each sequence; later rows
     are neither read nor counted, their h_seq is zero. ``h_seq_out`` / ``h_last_out``: tensors to write into;
-    ``h_last_out`` may be ``h_init`` itself (a decoder's state updated in place). Rows may be parts of wider ones (x and
+    ``h_last_out`` may be ``h_init`` itself (a decoder's state updated in place); otherwise they share no memory with the
+    inputs or each other. Rows may be parts of wider ones (x and
     gate as two halves of one projection); an innermost dimension that is not dense is copied first.
     """
     if not _is_plain(x_seq, gate_seq, gate, h_init, lengths, batch_first, state_dtype):
