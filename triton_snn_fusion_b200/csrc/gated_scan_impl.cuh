@@ -263,9 +263,6 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_kernel(const __gr
   const G g(q, dyn);
   const int T_ = (int)q.T, S = g.S;
   const bool leaky = LK == 1 || (LK == 2 && q.leaky);
-  Exchange<CH> cluster_maps;
-  if constexpr (SEG > 1)
-    cluster_maps.init(reinterpret_cast<float2 *>(dyn + (STAGED ? STAGES * G::STAGE : 0)), bars, &abort_flag, S, g.rank);
 
   // The state in front of the cluster's current tiles: with one segment each thread has its channels', otherwise the
   // first CH threads, the joiners, have one channel each.
@@ -285,6 +282,9 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_kernel(const __gr
   };
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) fetch((i * S + g.rank) * TC, i);
+  Exchange<CH> cluster_maps;
+  if constexpr (SEG > 1)      // behind every block's read of h_init: the first block may write h_last to the same buffer
+    cluster_maps.init(reinterpret_cast<float2 *>(dyn + (STAGED ? STAGES * G::STAGE : 0)), bars, &abort_flag, S, g.rank);
   int st = 0, base = 0, it = 0;
   // One tile. FULL: every step of it counts and all channels exist, so nothing is asked.
   auto work = [&](auto full) {
@@ -408,9 +408,6 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_backward_kernel(c
   const G g(q, dyn);
   const int T_ = (int)q.T, S = g.S;
   const bool leaky = LK == 1 || (LK == 2 && q.leaky);
-  Exchange<CH> cluster_maps;
-  if constexpr (SEG > 1)
-    cluster_maps.init(reinterpret_cast<float2 *>(dyn + (STAGED ? STAGES * G::STAGE : 0)), bars, &abort_flag, S, g.rank);
 
   // The first CH threads join the gradients of a channel each, the next CH threads the states. carry: the gradient that
   // reaches the cluster's current tiles from behind.
@@ -438,16 +435,21 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_backward_kernel(c
     if (tile0 == 0) state_load<T, CV>(q.h_init, q.state_f32, ji, jok && join_h, v);
     else if (tile0 > 0 && tile0 < g.len) state_load<float, CV>(q.ckpt, 1, (int64_t)(tile0 / kCkpt - 1) * q.B * q.D + ji, jok && join_h, v);
   };
-  int base = T_ > 0 ? (T_ - 1) / (S * TC) * (S * TC) : -1;
-  if constexpr (SEG > 1)      // tiles behind the sequence
-    for (; base >= g.len && base >= 0; base -= S * TC) {
-      g.zero(q.dx, base + g.rank * TC);
-      g.zero(q.dg, base + g.rank * TC);
-    }
+  const int last = T_ > 0 ? (T_ - 1) / (S * TC) * (S * TC) : -1;
+  int base = SEG == 1 ? last : g.len > 0 ? (g.len - 1) / (S * TC) * (S * TC) : -1;
   float front[CV] = {};
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) fetch(base - i * S * TC < 0 ? -1 : base + g.rank * TC - i * S * TC, i);
   front_of(base < 0 ? -1 : base + g.rank * TC, front);
+  Exchange<CH> cluster_maps;
+  if constexpr (SEG > 1) {
+    // behind every block's read of dh_last: the first block may write dh_init to the same buffer
+    cluster_maps.init(reinterpret_cast<float2 *>(dyn + (STAGED ? STAGES * G::STAGE : 0)), bars, &abort_flag, S, g.rank);
+    for (int t = last; t > base && t >= 0; t -= S * TC) {      // tiles behind the sequence
+      g.zero(q.dx, t + g.rank * TC);
+      g.zero(q.dg, t + g.rank * TC);
+    }
+  }
   int st = 0, it = 0;
   auto work = [&](auto full) {
     constexpr bool FULL = decltype(full)::value;
