@@ -309,3 +309,19 @@ def test_refusals_name_their_reason():
         ops.run_block_norm_backward(None, None, x)
     with pytest.raises(RuntimeError, match="dz is"):
         ops.run_block_norm_backward(x, x[:2], x)
+
+
+@gpu
+@pytest.mark.parametrize("M,D,row", [(3 * 444 * 16 + 8, 64, 8), (444 * 8 + 4, 63, 4)])
+def test_rows_behind_the_last_add_nothing_to_the_parameters(M, D, row):
+    """Several rows share a block, and in the last round some have none left: an infinite gradient of the row before makes an
+    infinite sum in its column, not NaN."""
+    v, dro, _ = _inputs(M, D, torch.bfloat16)
+    dro[row, 3] = float("inf")
+    r = ops.run_block_norm_backward(_dev(dro), None, _dev(v["y"]), gate=_dev(v["gate"]), residual=_dev(v["residual"]),
+                                    w_post=_dev(v["w_post"]), res_scale=_dev(v["res_scale"]), gate_act="silu", pre_norm=False)
+    q = float("inf") * float((v["y"][row, 3].float() * v["gate"][row, 3].float()).sign())
+    for got, w in ((r.dw_post, v["res_scale"]), (r.dres_scale, v["w_post"])):
+        assert float(got[3]) == q * float(w[3].float().sign())
+        got[3] = 0
+        assert bool(torch.isfinite(got).all())

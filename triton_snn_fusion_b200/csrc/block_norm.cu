@@ -355,11 +355,11 @@ __global__ void __launch_bounds__(TPR > 0 ? TPR : 128, MINB) block_norm_backward
   auto to_stage = [&](int st) {
     if constexpr (ST > 0) { y.p = slots + st * 5 * SLOT; g.p = y.p + SLOT; r.p = g.p + SLOT; o.p = r.p + SLOT; z.p = o.p + SLOT; }
   };
-  // a row that does not exist adds nothing to the column sums
+  // a row that does not exist adds nothing to the column sums: all of it is zero, for infinities of the row before it
+  // would make NaN of zeros
   auto fetch = [&](int64_t row) {
     if (row >= q.M) {
-      y.clear();
-      z.clear();
+      y.clear(); g.clear(); r.clear(); o.clear(); z.clear();
       return;
     }
     y.template load<ALL>(yp, stride * q.ys, step, in);
@@ -810,7 +810,6 @@ template <typename T> void launch_forward(NormArgs q, int dtype, cudaStream_t s)
   else if (p.nv == 4) { SNNB_NORM_BY_TPR(SNNB_CALL_1) }
   else block_norm_kernel<T, 1, 8, 512, 0><<<blocks, p.threads, 0, s>>>(q);
 #undef SNNB_CALL_V
-#undef SNNB_CALL_A
 #undef SNNB_CALL_1
 }
 
@@ -848,8 +847,7 @@ template <typename T> void launch_backward(NormArgs q, int dtype, cudaStream_t s
 #undef SNNB_CALL_V
 #undef SNNB_CALL_A
 #undef SNNB_CALL_1
-  if (q.dw_post || q.dscale || q.dw_pre)
-  {
+  if (q.dw_post || q.dscale || q.dw_pre) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((q.D + 31) / 32), 2);
     cfg.blockDim = dim3(1024);
