@@ -409,7 +409,7 @@ int snnb_block_norm_backward(const void *dres_out, int64_t dres_out_stride, cons
  *   high (k odd) half of byte k / 2; scales [N][ceil(K / G)] and bias [N] (or NULL) in the x dtype; zeros
  *   [N][ceil(K / G)] uint8, at most 127, or NULL (8 everywhere); y [M][N], rows y_stride elements apart,
  *   apart from x.
- * K % 32 == 0, G 32, 64 or 128; the last group may be shorter than G. N * K < 2^33, M <= 131070. The weights are read
+ * K % 32 == 0, G 32, 64 or 128; the last group may be shorter than G. K <= 2^30, N * K < 2^33, M <= 131070. The weights are read
  * once for every 32 tokens (fp32: 10), so beyond some hundred tokens a product over widened weights is the faster way.
  */
 int snnb_linear_w4(const void *x, int64_t x_stride, const void *q_weight, const void *scales, const void *zeros,

@@ -193,3 +193,26 @@ def test_refusals_name_their_reason():
                            ((x, q[:0], s[:0]), dict(group_size=32), "no rows"), (([x], q, s), {}, "expected a Tensor")):
         with pytest.raises(RuntimeError, match=text):
             ops.run_linear_w4(*args, **kw)
+
+
+def test_sizes_whose_offsets_would_wrap_are_refused():
+    """A row of 2^31 - 32 weights: the step behind its last one has no 32-bit number. The addresses are never read."""
+    for K in (2 ** 31 - 32, 2 ** 30 + 32):
+        assert _lib.lib.snnb_linear_w4(4096, K, 4096, 4096, None, None, 8192, 1, 1, K, 1, 128, _lib.F32, None) == 1
+        assert b"too large" in _lib.lib.snnb_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [1, 12, 40])
+def test_infinite_tokens(dtype, M):
+    """An infinite value gives infinities of the weight's sign, and no number only where that weight is zero."""
+    K, N, G = 256, 40, 64
+    x, q, s, z, b = _inputs(M, K, N, G, dtype)
+    for k, v in ((100, float("inf")), (255, -float("inf")), (0, float("inf"))):
+        x2 = x.clone()
+        x2[M // 2, k] = v
+        y = ops.run_linear_w4(_dev(x2), _dev(q), _dev(s), _dev(z), _dev(b), group_size=G)[M // 2].double().cpu()
+        weight = (q[:, k // 2] >> (4 * (k % 2)) & 15).double() - z[:, k // G].double()
+        want = weight * v
+        assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.nan_to_num(nan=0.0, posinf=2, neginf=-2), want.nan_to_num(nan=0.0, posinf=2, neginf=-2))

@@ -134,7 +134,7 @@ __device__ __forceinline__ void fill_x(const W4Args &a, int64_t m0, int tokens, 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float f = in ? src[e] : 0.f;
-          const float hi = __uint_as_float(__float_as_uint(f) & 0xffff0000u), r1 = f - hi;
+          const float hi = __uint_as_float(__float_as_uint(f) & 0xffff0000u), r1 = f == hi ? 0.f : f - hi;      // also of infinities
           const float mid = __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
           const float part[3] = {hi, mid, r1 - mid};
 #pragma unroll
@@ -393,7 +393,7 @@ extern "C" int snnb_linear_w4(const void *x, int64_t x_stride, const void *q_wei
   SNNB_CHECK_ARG(group_size == 32 || group_size == 64 || group_size == 128, "linear_w4: groups of 32, 64 or 128 values, got %d",
                  group_size);
   if (K % 32 != 0) return fail(SNNB_ERR_UNSUPPORTED, "linear_w4: K must be a multiple of 32, got %d", K);
-  SNNB_CHECK_ARG((int64_t)N * K < (1LL << 33) && M <= 65535 * 2, "linear_w4: problem too large");
+  SNNB_CHECK_ARG(K <= (1 << 30) && (int64_t)N * K < (1LL << 33) && M <= 65535 * 2, "linear_w4: problem too large");
   if (M == 0) return SNNB_OK;
   SNNB_CHECK_ARG(x && q_weight && scales && y, "linear_w4: null pointer");
   SNNB_CHECK_ARG(x_stride >= 0 && (M <= 1 || y_stride >= N), "linear_w4: bad row stride");

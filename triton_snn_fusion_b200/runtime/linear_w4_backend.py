@@ -119,7 +119,7 @@ def run_linear_w4(
     verbose: bool = False,
 ) -> torch.Tensor:
     """x [..., K] -> [..., N] in x's dtype. ``q_weight``, ``scales`` and ``zeros`` as ``quantize_linear_w4`` lays them out;
-    keep them contiguous (they are copied at every call otherwise). ``out``: a contiguous tensor to write into."""
+    keep them contiguous (they are copied at every call otherwise). ``out``: a contiguous tensor to write into, apart from x."""
     if not _is_plain(x, q_weight, scales, zeros, bias, group_size):
         raise_reasons("linear_w4", check_linear_w4_support(x, q_weight, scales, zeros, bias, group_size), False, verbose)
     K, N = int(x.shape[-1]), int(q_weight.shape[0])
