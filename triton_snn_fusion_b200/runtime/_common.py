@@ -178,7 +178,7 @@ def rows_2d(t: torch.Tensor) -> torch.Tensor:
 
 def dense_like(t: torch.Tensor) -> torch.Tensor:
     """Uninitialised contiguous tensor of t's shape, type and device."""
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def launch(symbol: str, device: torch.device, *args) -> None:

@@ -208,11 +208,11 @@ def run_block_norm_backward(
     dy, dgate = dense_like(lead) if y is not None else None, dense_like(lead) if gate is not None else None
     dres = dense_like(lead)
     # without rows, or without a gradient of z, a sum is empty
-    sums = (torch.empty if M > 0 and dz is not None else torch.zeros)((3, D), dtype=torch.float32, device=lead.device).unbind(0)
+    sums = (lead.new_empty if M > 0 and dz is not None else lead.new_zeros)((3, D), dtype=torch.float32).unbind(0)
     dw_post, dscale, dw_pre = (s if w is not None else None for s, w in zip(sums, (w_post, res_scale, w_pre)))
     if M > 0:
         (wp, sc, wr), w_code = _params(lead, w_post, res_scale, w_pre)
-        ws = torch.empty(_lib.lib.snnb_block_norm_backward_workspace_bytes(M, D), dtype=torch.uint8, device=lead.device)
+        ws = lead.new_empty(_lib.lib.snnb_block_norm_backward_workspace_bytes(M, D), dtype=torch.uint8)
         k0, dop, dos = _rows(dres_out)
         k1, dzp, dzs = _rows(dz)
         k2, yp, ys = _rows(y)

@@ -125,7 +125,7 @@ def run_linear_w4(
     K, N = int(x.shape[-1]), int(q_weight.shape[0])
     shape = (*x.shape[:-1], N)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(shape)
     elif tuple(out.shape) != shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
         raise RuntimeError(f"unsupported_output: out must be a contiguous {x.dtype} tensor of shape {shape} on {x.device}")
     M = x.numel() // K

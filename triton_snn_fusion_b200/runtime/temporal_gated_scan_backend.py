@@ -87,9 +87,9 @@ def _strides(t, batch_first):
     return (s[1], s[0]) if batch_first else (s[0], s[1])
 
 
-def _state_out(name, t, B, D, dtype, x_seq):
+def _state_out(name, t, B, D, dtype, x_seq, like=None):
     if t is None:
-        return torch.empty((B, D), dtype=dtype, device=x_seq.device)
+        return torch.empty_like(like) if like is not None else x_seq.new_empty((B, D), dtype=dtype)
     if tuple(t.shape) != (B, D) or t.dtype != dtype or t.device != x_seq.device or not t.is_contiguous():
         raise RuntimeError(f"unsupported_output: {name} must be a contiguous {dtype} tensor of shape {(B, D)} on {x_seq.device}")
     return t
@@ -137,7 +137,7 @@ def run_temporal_gated_scan(
         if h.shape != x.shape or h.dtype != x.dtype or h.device != x.device or (D > 1 and h.stride(2) != 1):
             raise RuntimeError(f"unsupported_output: h_seq_out must be a {x.dtype} tensor of shape {tuple(x.shape)} with "
                                f"dense rows on {x.device}")
-    h_last = _state_out("h_last_out", h_last_out, B, D, s_dt, x)
+    h_last = _state_out("h_last_out", h_last_out, B, D, s_dt, x, h0)
     ckpt = None
     if save_for_backward:
         ckpt = torch.empty((_lib.lib.snnb_gated_scan_ckpt_rows(T), B, D), dtype=torch.float32, device=x.device)
@@ -190,7 +190,7 @@ def run_temporal_gated_scan_backward(
     dl = dl.contiguous() if dl is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
     dx, dg = dense_like(x), dense_like(x)
-    dh_init = torch.empty((B, D), dtype=s_dt, device=x.device)
+    dh_init = _state_out("dh_init", None, B, D, s_dt, x, h0)
     launch("snnb_gated_scan_backward", x.device,
            dh.data_ptr(), *_strides(dh, batch_first), _lib.ptr(dl), x.data_ptr(), *_strides(x, batch_first),
            g.data_ptr(), *_strides(g, batch_first), _lib.ptr(h0), _lib.ptr(ckpt), _lib.ptr(lengths),
