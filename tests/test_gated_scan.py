@@ -87,6 +87,19 @@ def test_padded_batches(batch_first, D):
 
 
 @gpu
+@pytest.mark.parametrize("T", [10, 15, 16, 17, 24, 40, 63, 64, 65])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_short_tiles(T, dtype):
+    """Sequences of one short tile, whole and padded, with the last channels of a tile missing and with rows that start
+    anywhere."""
+    n = [0, 1, 8, 9, T - 1, T, T + 3]
+    for D in (200, 75):
+        for kind, leaky in (("sigmoid", True), ("value", False)):
+            _check(T, len(n), D, dtype, kind, leaky, lengths=n, batch_first=D == 200, seed=T)
+            _check(T, 3, D, dtype, kind, leaky, batch_first=D == 75, state=dtype, seed=T + 1)
+
+
+@gpu
 def test_padding_is_not_read():
     T, B, D = 300, 3, 72
     n = torch.tensor([0, 17, 200], dtype=torch.int32)

@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_backward_kernel(c
   constexpr int CH = G::CH, TC = G::TC, SZ = G::SZ;
   constexpr bool STAGED = R == Rows::copied;
   static_assert(SEG == 1 || 2 * CH <= LANES * SEG, "two threads per channel");
-  static_assert(SEG == 1 || TC == kCkpt || TC == 32, "a tile starts from a checkpoint, or is the only one");
+  static_assert(SEG == 1 || TC == kCkpt || TC <= 64, "a tile starts from a checkpoint, or is the only one");
   __shared__ __align__(16) float sA[SEG > 1 ? SEG * CH : 4], sH[SEG > 1 ? SEG * CH : 4], sC[SEG > 1 ? SEG * CH : 4];
   __shared__ uint64_t bars[2];
   __shared__ int abort_flag;
@@ -668,19 +668,40 @@ int scan_cluster(int64_t tiles, int64_t steps) {
   return S;
 }
 
-// Up to 8 steps a thread walks alone, up to 32 the loads go straight to registers in few segments. Beyond that:
-// - rows on 16-byte boundaries: tiles of 64 bytes of channels x 128 steps, two of them in shared memory, 128 threads with 8
+// Up to 8 steps a thread walks alone. Beyond that:
+// - rows on 16-byte boundaries, up to 64 steps: one tile, no longer than needed, through shared memory. Measured against
+//   the tile of 32 steps straight to registers and, from 33 steps on, the tile of 128 (bf16, D2048, us, forward and
+//   backward): T16 B256 23 43 instead of 41 64, T24 B160 25 41 instead of 31 45, T33 B128 33 49 instead of 51 80, T64 B64
+//   21 29 instead of 31 47. At T100 and T128 a single stage is no faster than the two of the long form (27 37 to 25 38).
+// - the same, longer: tiles of 64 bytes of channels x 128 steps, two of them in shared memory, 128 threads with 8
 //   steps of 8 bytes each and four blocks to an SM. Wider tiles leave too few blocks (64 channels, 256 threads: 71 us
 //   instead of 47 for B8 T2048 D2048 bf16), 4 steps a thread double the joining (61 us); the backward pass with three
 //   blocks and three tiles in shared memory took 86 us instead of 77, its 512 blocks then being more than run at once.
-// - ragged rows: nothing wider than a value can be loaded, so the loads of many warps hide each other instead (64
-//   registers, 32 warps to an SM): 95 us forward and 204 backward for B8 T2048 D2047 bf16. Copying the 16-byte blocks or
-//   the words that a row lies in took 106 and 152 us: the addresses cost more than the loads.
+// - ragged rows: up to 32 steps one tile. Nothing wider than a value can be loaded, so the loads of many warps hide each
+//   other instead (64 registers, 32 warps to an SM): 95 us forward and 204 backward for B8 T2048 D2047 bf16. Copying the
+//   16-byte blocks or the words that a row lies in took 106 and 152 us: the addresses cost more than the loads.
+template <typename T, bool SIG, int SEG, int L> int forward_tile(const ScanArgs &q, cudaStream_t s) {
+  constexpr int VEC = 8 / (int)sizeof(T);
+  using G = Tile<T, Rows::copied, VEC, 8, SEG, L, 1, 2>;
+  return launch_tiles<gated_scan_kernel<T, Rows::copied, SIG, 2, VEC, 8, SEG, L, 1, 64 / SEG>>(q, 8 * SEG, G::CH, 1, G::STAGE, s);
+}
+template <typename T, bool SIG, int SEG, int L> int backward_tile(const ScanArgs &q, cudaStream_t s) {
+  constexpr int VEC = 8 / (int)sizeof(T);
+  using G = Tile<T, Rows::copied, VEC, 8, SEG, L, 1, 3>;
+  return launch_tiles<gated_scan_backward_kernel<T, Rows::copied, SIG, 2, VEC, 8, SEG, L, 1, 64 / SEG>>(q, 8 * SEG, G::CH, 1, G::STAGE, s);
+}
+
 template <typename T, bool SIG, Rows R> int forward(const ScanArgs &q, cudaStream_t s) {
-  constexpr int VEC = R == Rows::ragged ? 1 : 8 / (int)sizeof(T), W = VEC > 1 ? 16 : 32;
+  constexpr int VEC = R == Rows::ragged ? 1 : 8 / (int)sizeof(T);
   if (q.T <= 1) return launch_tiles<gated_scan_kernel<T, R == Rows::ragged ? Rows::ragged : Rows::direct, SIG, 2, VEC, 64, 1, 1, 1, 1>>(q, 64, 64 * VEC, 1, 0, s);
   if (q.T <= 8) return launch_tiles<gated_scan_kernel<T, R == Rows::ragged ? Rows::ragged : Rows::direct, SIG, 2, VEC, 64, 1, 8, 1, 1>>(q, 64, 64 * VEC, 1, 0, s);
-  if (q.T <= 32) return launch_tiles<gated_scan_kernel<T, R == Rows::ragged ? Rows::ragged : Rows::direct, SIG, 2, VEC, W, 4, 8, 1, 1>>(q, W * 4, W * VEC, 1, 0, s);
+  if constexpr (R == Rows::copied) {
+    if (q.T <= 16) return forward_tile<T, SIG, 4, 4>(q, s);
+    if (q.T <= 32) return forward_tile<T, SIG, 4, 8>(q, s);
+    if (q.T <= 64) return forward_tile<T, SIG, 8, 8>(q, s);
+  } else {
+    if (q.T <= 32) return launch_tiles<gated_scan_kernel<T, R, SIG, 2, 1, 32, 4, 8, 1, 1>>(q, 128, 32, 1, 0, s);
+  }
   constexpr bool RAG = R == Rows::ragged;
   constexpr int V = RAG ? 2 : VEC, LANES = RAG ? 16 : 8, SEG = 16, L = RAG ? 4 : 8, ST = RAG ? 0 : 2, MINB = 4;
   using G = Tile<T, R, V, LANES, SEG, L, ST, 2>;
@@ -691,9 +712,15 @@ template <typename T, bool SIG, Rows R> int forward(const ScanArgs &q, cudaStrea
 }
 
 template <typename T, bool SIG, Rows R> int backward(const ScanArgs &q, cudaStream_t s) {
-  constexpr int VEC = R == Rows::ragged ? 1 : 8 / (int)sizeof(T), W = VEC > 1 ? 16 : 32;
+  constexpr int VEC = R == Rows::ragged ? 1 : 8 / (int)sizeof(T);
   if (q.T <= 8) return launch_tiles<gated_scan_backward_kernel<T, R == Rows::ragged ? Rows::ragged : Rows::direct, SIG, 2, VEC, 64, 1, 8, 1, 1>>(q, 64, 64 * VEC, 1, 0, s);
-  if (q.T <= 32) return launch_tiles<gated_scan_backward_kernel<T, R == Rows::ragged ? Rows::ragged : Rows::direct, SIG, 2, VEC, W, 8, 4, 1, 1>>(q, W * 8, W * VEC, 1, 0, s);
+  if constexpr (R == Rows::copied) {
+    if (q.T <= 16) return backward_tile<T, SIG, 8, 2>(q, s);
+    if (q.T <= 32) return backward_tile<T, SIG, 8, 4>(q, s);
+    if (q.T <= 64) return backward_tile<T, SIG, 8, 8>(q, s);
+  } else {
+    if (q.T <= 32) return launch_tiles<gated_scan_backward_kernel<T, R, SIG, 2, 1, 32, 8, 4, 1, 1>>(q, 256, 32, 1, 0, s);
+  }
   constexpr bool RAG = R == Rows::ragged;
   constexpr int V = RAG ? 2 : VEC, LANES = RAG ? 16 : 8, SEG = RAG ? 32 : 16, L = RAG ? 4 : 8, ST = RAG ? 0 : 2, MINB = RAG ? 2 : 4;
   using G = Tile<T, R, V, LANES, SEG, L, ST, 3>;
