@@ -6,6 +6,9 @@
     python -m triton_snn_fusion_b200.microbench tail --B 256 --c 1024 --hw 7 --classes 1000
     python -m triton_snn_fusion_b200.microbench stem --B 128 --hw 224
     python -m triton_snn_fusion_b200.microbench linear --M 4096 --K 768 --N 3072
+    python -m triton_snn_fusion_b200.microbench scan --T 2048 --B 8 --D 2048 --backward 1
+    python -m triton_snn_fusion_b200.microbench norm --M 16384 --D 2048 --backward 1
+    python -m triton_snn_fusion_b200.microbench w4 --M 1 --K 8192 --N 16384
     python -m triton_snn_fusion_b200.microbench mma                # cycles per tcgen05.mma for M x N shapes
 
 Each case builds seeded synthetic spikes/currents on the GPU (larger than L2 at the default sizes),
@@ -24,6 +27,7 @@ import torch
 from . import _lib
 
 DEV = "cuda"
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 LIF = (1.0, 0.0, 2.0)   # v_th, v_reset, tau: the reference's defaults
 
 
@@ -199,6 +203,46 @@ def case_stem(a):
           f"{nbytes / ms / 1e6:.0f} GB/s  spike rate {rate:.3f}  device status {_lib.device_status()}")
 
 
+def _report(name, a, fwd, bwd, values):
+    ms = _time(fwd, a.reps)
+    print(f"{name} {a.dtype}: {ms:.4f} ms  {values[0] / ms / 1e6:.0f} GB/s")
+    if a.backward:
+        ms = _time(bwd, a.reps)
+        print(f"{name} {a.dtype} backward: {ms:.4f} ms  {values[1] / ms / 1e6:.0f} GB/s")
+
+
+def case_scan(a):
+    from .runtime.temporal_gated_scan_backend import run_temporal_gated_scan, run_temporal_gated_scan_backward
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x, gate, dh = (torch.randn(a.B, a.T, a.D, device=DEV, generator=g).to(DTYPES[a.dtype]) for _ in range(3))
+    ckpt = run_temporal_gated_scan(x, gate, batch_first=True, save_for_backward=True).ckpt
+    n = x.numel() * x.element_size()
+    _report(f"gated_scan T{a.T} B{a.B} D{a.D}", a, lambda: run_temporal_gated_scan(x, gate, batch_first=True),
+            lambda: run_temporal_gated_scan_backward(dh, x, gate, None, ckpt, batch_first=True), (3 * n, 5 * n))
+    print(f"device status {_lib.device_status()}")
+
+
+def case_norm(a):
+    from .runtime.block_norm_backend import run_block_norm, run_block_norm_backward
+    g = torch.Generator(device=DEV).manual_seed(0)
+    y, gate, res, do, dz = (torch.randn(a.M, a.D, device=DEV, generator=g).to(DTYPES[a.dtype]) for _ in range(5))
+    w = {k: torch.randn(a.D, device=DEV, generator=g).to(y.dtype) for k in ("w_post", "res_scale", "w_pre")}
+    n = y.numel() * y.element_size()
+    _report(f"block_norm M{a.M} D{a.D}", a, lambda: run_block_norm(y, gate=gate, residual=res, gate_act="silu", **w),
+            lambda: run_block_norm_backward(do, dz, y, gate=gate, residual=res, gate_act="silu", **w), (5 * n, 8 * n))
+
+
+def case_w4(a):
+    from .runtime.linear_w4_backend import quantize_linear_w4, run_linear_w4
+    g = torch.Generator(device=DEV).manual_seed(0)
+    q = quantize_linear_w4(torch.randn(a.N, a.K, device=DEV, generator=g).to(DTYPES[a.dtype]), a.group)
+    x = torch.randn(a.M, a.K, device=DEV, generator=g).to(DTYPES[a.dtype])
+    ms = _time(lambda: run_linear_w4(x, *q, group_size=a.group), a.reps)
+    nbytes = a.N * a.K / 2 + q.scales.numel() * q.scales.element_size() + (x.numel() + a.M * a.N) * x.element_size()
+    print(f"linear_w4 M{a.M} {a.K}->{a.N} G{a.group} {a.dtype}: {ms:.4f} ms  {nbytes / ms / 1e6:.0f} GB/s  "
+          f"{2.0 * a.M * a.N * a.K / ms / 1e9:.1f} TFLOP/s")
+
+
 def case_mma(a):
     """SM cycles per tcgen05.mma (K = 16, bf16, fp32 accumulate) for the shapes the tile layouts choose between,
     with one block on the GPU and with one block on every SM; then the 128 x 256 shape on every SM for about 0.2 s
@@ -287,6 +331,26 @@ def main(argv=None):
     n.add_argument("--path", type=int, default=_lib.PATH_TCGEN05)
     n.add_argument("--dist", choices=["bernoulli", "normal"], default="bernoulli")
     n.set_defaults(fn=case_linear)
+    sc = sub.add_parser("scan")
+    sc.add_argument("--T", type=int, default=2048)
+    sc.add_argument("--B", type=int, default=8)
+    sc.add_argument("--D", type=int, default=2048)
+    sc.set_defaults(fn=case_scan)
+    no = sub.add_parser("norm")
+    no.add_argument("--M", type=int, default=16384)
+    no.add_argument("--D", type=int, default=2048)
+    no.set_defaults(fn=case_norm)
+    w4 = sub.add_parser("w4")
+    w4.add_argument("--M", type=int, default=1)
+    w4.add_argument("--K", type=int, default=8192)
+    w4.add_argument("--N", type=int, default=16384)
+    w4.add_argument("--group", type=int, choices=[32, 64, 128], default=128)
+    w4.set_defaults(fn=case_w4)
+    for p in (sc, no, w4):
+        p.add_argument("--dtype", choices=sorted(DTYPES), default="bf16")
+        p.add_argument("--reps", type=int, default=10)
+    for p in (sc, no):
+        p.add_argument("--backward", type=int, default=0)
     q = sub.add_parser("mma")
     q.add_argument("--reps-mma", type=int, default=512, help="batches of four MMAs per measurement")
     q.set_defaults(fn=case_mma)
