@@ -75,11 +75,18 @@ def check_temporal_gated_scan_support(x_seq, gate_seq, h_init, gate, lengths=Non
 def _is_plain(x, g, gate, h0, lengths, batch_first, state_dtype) -> bool:
     """Whether nothing needs a second look: what ``check_temporal_gated_scan_support`` would say yes to, at the price that a
     decoding step can pay. Anything else goes through the full check."""
-    return (type(x) is torch.Tensor and type(g) is torch.Tensor and x.is_cuda and x.dim() == 3 and x.dtype in ACT_DTYPES
+    if not (type(x) is torch.Tensor and type(g) is torch.Tensor and x.is_cuda and x.dim() == 3 and x.dtype in ACT_DTYPES
             and g.shape == x.shape and g.dtype == x.dtype and g.device == x.device and gate in GATES
-            and (h0 is None or (type(h0) is torch.Tensor and h0.dtype == torch.float32 and h0.device == x.device
-                                and h0.shape == (x.shape[0 if batch_first else 1], x.shape[2])))
-            and lengths is None and state_dtype is None)
+            and state_dtype in (None, torch.float32)):
+        return False
+    B, D = x.shape[0 if batch_first else 1], x.shape[2]
+    return ((h0 is None or _is_f32(h0, (B, D), x.device))
+            and (lengths is None or (type(lengths) is torch.Tensor and lengths.dtype == torch.int32
+                                     and lengths.device == x.device and lengths.shape == (B,))))
+
+
+def _is_f32(t, shape, device) -> bool:
+    return type(t) is torch.Tensor and t.dtype == torch.float32 and t.device == device and t.shape == shape
 
 
 def _strides(t, batch_first):
@@ -148,6 +155,32 @@ def run_temporal_gated_scan(
     return TemporalGatedScanResult(h, h_last, ckpt)
 
 
+def _is_ckpt(ckpt, x, batch_first) -> bool:
+    T, B, D = _sizes(x, batch_first)
+    rows = _lib.lib.snnb_gated_scan_ckpt_rows(T)
+    return (ckpt is None and rows == 0) or (_is_f32(ckpt, (rows, B, D), x.device) and ckpt.is_contiguous())
+
+
+def _check_backward(dh_seq, x_seq, gate_seq, h_init, ckpt, dh_last, gate, lengths, batch_first) -> List[str]:
+    why = check_temporal_gated_scan_support(x_seq, gate_seq, h_init, gate, lengths, batch_first)
+    if isinstance(x_seq, torch.Tensor) and x_seq.dim() == 3:
+        T, B, D = _sizes(x_seq, batch_first)
+        g = Gate("x_seq", x_seq)
+        _like(g, "dh_seq", dh_seq, x_seq.shape)
+        h0, dl = state_or_none(h_init), state_or_none(dh_last)
+        if dl is not None:
+            _like(g, "dh_last", dl, (B, D), h0.dtype if h0 is not None else dl.dtype)
+            if dl.dtype not in (x_seq.dtype, torch.float32):
+                g.add("unsupported_dtype", f"dh_last is {dl.dtype}, the state is {x_seq.dtype} or torch.float32")
+        rows = _lib.lib.snnb_gated_scan_ckpt_rows(T)
+        if ckpt is not None or rows > 0:
+            _like(g, "ckpt", ckpt, (rows, B, D), torch.float32)
+            if isinstance(ckpt, torch.Tensor) and not ckpt.is_contiguous():
+                g.add("unsupported_layout", "ckpt is not contiguous")
+        why += g.why
+    return why
+
+
 def run_temporal_gated_scan_backward(
     dh_seq: torch.Tensor,
     x_seq: torch.Tensor,
@@ -167,23 +200,14 @@ def run_temporal_gated_scan_backward(
     The other arguments are those of the forward call and the ``ckpt`` that it returned; x_seq, gate_seq and h_init must
     hold what they held then. dh_init has the state's dtype: h_init's, without one dh_last's, else fp32.
     """
-    why = check_temporal_gated_scan_support(x_seq, gate_seq, h_init, gate, lengths, batch_first)
-    if isinstance(x_seq, torch.Tensor) and x_seq.dim() == 3:
-        T, B, D = _sizes(x_seq, batch_first)
-        g = Gate("x_seq", x_seq)
-        _like(g, "dh_seq", dh_seq, x_seq.shape)
-        h0, dl = state_or_none(h_init), state_or_none(dh_last)
-        if dl is not None:
-            _like(g, "dh_last", dl, (B, D), h0.dtype if h0 is not None else dl.dtype)
-            if dl.dtype not in (x_seq.dtype, torch.float32):
-                g.add("unsupported_dtype", f"dh_last is {dl.dtype}, the state is {x_seq.dtype} or torch.float32")
-        rows = _lib.lib.snnb_gated_scan_ckpt_rows(T)
-        if ckpt is not None or rows > 0:
-            _like(g, "ckpt", ckpt, (rows, B, D), torch.float32)
-            if isinstance(ckpt, torch.Tensor) and not ckpt.is_contiguous():
-                g.add("unsupported_layout", "ckpt is not contiguous")
-        why += g.why
-    raise_reasons("temporal_gated_scan_backward", why, False, verbose)
+    if not (_is_plain(x_seq, gate_seq, gate, h_init, lengths, batch_first, None) and type(dh_seq) is torch.Tensor
+            and dh_seq.shape == x_seq.shape and dh_seq.dtype == x_seq.dtype and dh_seq.device == x_seq.device
+            and (dh_last is None or _is_f32(dh_last, (x_seq.shape[0 if batch_first else 1], x_seq.shape[2]), x_seq.device))
+            and _is_ckpt(ckpt, x_seq, batch_first)):
+        raise_reasons("temporal_gated_scan_backward",
+                      _check_backward(dh_seq, x_seq, gate_seq, h_init, ckpt, dh_last, gate, lengths, batch_first), False, verbose)
+    T, B, D = _sizes(x_seq, batch_first)
+    h0, dl = state_or_none(h_init), state_or_none(dh_last)
     dh, x, g = rows_dense(dh_seq), rows_dense(x_seq), rows_dense(gate_seq)
     s_dt = h0.dtype if h0 is not None else (dl.dtype if dl is not None else torch.float32)
     h0 = h0.contiguous() if h0 is not None else None
