@@ -314,8 +314,10 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_kernel(const __gr
           widen<T, VEC>(g.slot(0, st, l)->v, gv);
           widen<T, VEC>(g.slot(1, st, l)->v, u[l]);
         } else {
-          widen<T, VEC>(in[l][0].v, gv);
-          widen<T, VEC>(in[l][1].v, u[l]);
+          // (ragged rows one by one: 96 us instead of 139 for B8 T2048 D2047 bf16; the backward pass, which keeps them
+          // longer, is faster with words: 104 instead of 117 for B64 T64 D2047)
+          widen<T, VEC, R != Rows::ragged>(in[l][0].v, gv);
+          widen<T, VEC, R != Rows::ragged>(in[l][1].v, u[l]);
         }
         gates_of<SIG, VEC>(gv, a[l], bb);
         if (leaky) v_mul(bb, u[l], u[l]);
@@ -677,9 +679,12 @@ int scan_cluster(int64_t tiles, int64_t steps) {
 //   steps of 8 bytes each and four blocks to an SM. Wider tiles leave too few blocks (64 channels, 256 threads: 71 us
 //   instead of 47 for B8 T2048 D2048 bf16), 4 steps a thread double the joining (61 us); the backward pass with three
 //   blocks and three tiles in shared memory took 86 us instead of 77, its 512 blocks then being more than run at once.
-// - ragged rows: up to 32 steps one tile. Nothing wider than a value can be loaded, so the loads of many warps hide each
-//   other instead (64 registers, 32 warps to an SM): 95 us forward and 204 backward for B8 T2048 D2047 bf16. Copying the
-//   16-byte blocks or the words that a row lies in took 106 and 152 us: the addresses cost more than the loads.
+// - ragged rows: nothing wider than a value can be loaded, so the loads of many warps hide each other instead (64
+//   registers, 32 warps to an SM): 96 us forward and 199 backward for B8 T2048 D2047 bf16. Copying the 16-byte blocks or
+//   the words that a row lies in took 106 and 152 us: the addresses cost more than the loads; loading a tile ahead into
+//   registers took as long. Up to 32 steps, backward 64, one tile no longer than needed, 4 steps a thread: 25 and 39 us for
+//   T16 B256 D2047, 27 and 41 for T64 B64; with 8 steps of one channel a thread in 128 threads 139 and 152, in the long
+//   form 104 backward for T64 B64.
 template <typename T, bool SIG, int SEG, int L> int forward_tile(const ScanArgs &q, cudaStream_t s) {
   constexpr int VEC = 8 / (int)sizeof(T);
   using G = Tile<T, Rows::copied, VEC, 8, SEG, L, 1, 2>;
@@ -700,7 +705,8 @@ template <typename T, bool SIG, Rows R> int forward(const ScanArgs &q, cudaStrea
     if (q.T <= 32) return forward_tile<T, SIG, 4, 8>(q, s);
     if (q.T <= 64) return forward_tile<T, SIG, 8, 8>(q, s);
   } else {
-    if (q.T <= 32) return launch_tiles<gated_scan_kernel<T, R, SIG, 2, 1, 32, 4, 8, 1, 1>>(q, 128, 32, 1, 0, s);
+    if (q.T <= 16) return launch_tiles<gated_scan_kernel<T, R, SIG, 2, 2, 16, 4, 4, 0, 16>>(q, 64, 32, 1, 0, s);
+    if (q.T <= 32) return launch_tiles<gated_scan_kernel<T, R, SIG, 2, 2, 16, 8, 4, 0, 8>>(q, 128, 32, 1, 0, s);
   }
   constexpr bool RAG = R == Rows::ragged;
   constexpr int V = RAG ? 2 : VEC, LANES = RAG ? 16 : 8, SEG = 16, L = RAG ? 4 : 8, ST = RAG ? 0 : 2, MINB = 4;
@@ -719,7 +725,9 @@ template <typename T, bool SIG, Rows R> int backward(const ScanArgs &q, cudaStre
     if (q.T <= 32) return backward_tile<T, SIG, 8, 4>(q, s);
     if (q.T <= 64) return backward_tile<T, SIG, 8, 8>(q, s);
   } else {
-    if (q.T <= 32) return launch_tiles<gated_scan_backward_kernel<T, R, SIG, 2, 1, 32, 8, 4, 1, 1>>(q, 256, 32, 1, 0, s);
+    if (q.T <= 16) return launch_tiles<gated_scan_backward_kernel<T, R, SIG, 2, 2, 16, 4, 4, 0, 16>>(q, 64, 32, 1, 0, s);
+    if (q.T <= 32) return launch_tiles<gated_scan_backward_kernel<T, R, SIG, 2, 2, 16, 8, 4, 0, 8>>(q, 128, 32, 1, 0, s);
+    if (q.T <= 64) return launch_tiles<gated_scan_backward_kernel<T, R, SIG, 2, 2, 16, 16, 4, 0, 4>>(q, 256, 32, 1, 0, s);
   }
   constexpr bool RAG = R == Rows::ragged;
   constexpr int V = RAG ? 2 : VEC, LANES = RAG ? 16 : 8, SEG = RAG ? 32 : 16, L = RAG ? 4 : 8, ST = RAG ? 0 : 2, MINB = RAG ? 2 : 4;

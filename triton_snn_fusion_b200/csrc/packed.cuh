@@ -59,9 +59,10 @@ template <int N> __device__ __forceinline__ void v_set(float (&r)[N], float v) {
 }
 
 // p: the start of a Pack<T, N> (its alignment is what allows whole words). A bf16 is the upper half of an fp32: one
-// instruction a value from the word that holds two.
-template <typename T, int N> __device__ __forceinline__ void widen(const T *p, float (&v)[N]) {
-  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+// instruction a value from the word that holds two. WORDS false: the values were loaded one by one, and a word would have
+// to be put together first, which waits for the loads.
+template <typename T, int N, bool WORDS = true> __device__ __forceinline__ void widen(const T *p, float (&v)[N]) {
+  if constexpr (WORDS && sizeof(T) == 2 && N % 2 == 0) {
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
       const uint32_t w = *reinterpret_cast<const uint32_t *>(p + k);
