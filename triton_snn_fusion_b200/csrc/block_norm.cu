@@ -727,8 +727,8 @@ __global__ void __launch_bounds__(1024) block_norm_sums_kernel(const __grid_cons
 // 70 us instead of 61 (16384 rows of 2048 bf16 values), and the backward pass has no registers for them. Two pieces only
 // where 512 threads with one do not reach (up to 8192 16-bit or 4096 fp32 columns), single columns where rows do not start
 // on 16-byte boundaries (4096 rows of 2047 bf16 values: forward 2.4 TB/s, backward 1.1; loading a row ahead into registers
-// changed nothing), and the long-row kernel (1.1 TB/s backward at 16384 columns, rows being read five times) behind that. Laid over threads: `vec` columns (16 bytes, or one where rows do not start on 16-byte boundaries) in
-// `nv` pieces for each of tpr threads; nv = 0: the long-row kernel.
+// changed nothing), and the long-row kernel (1.1 TB/s backward at 16384 columns, rows being read five times) behind that.
+// A plan: `vec` columns in `nv` pieces for each of tpr threads; nv = 0: the long-row kernel.
 struct Plan { int vec, nv, tpr, threads; };
 Plan plan_of(int D, int dtype, bool aligned) {
   Plan p;

@@ -64,9 +64,8 @@ int dispatch(ScanArgs q, bool backward, int gate_kind, int dtype, cudaStream_t s
   }
   if (q.B == 1) q.x.bs = q.g.bs = q.h.bs = q.dx.bs = q.dg.bs = 0;
   const int sz = dtype_size(dtype);
-  auto state16 = [](const void *p) { return aligned16(p); };
-  const bool aligned = q.D % (16 / sz) == 0 && state16(q.h_init) && state16(q.dh_last) && state16(q.h_last) && rows16(q.x, sz) && rows16(q.g, sz) && rows16(q.h, sz) && rows16(q.dx, sz) &&
-                   rows16(q.dg, sz);
+  const bool aligned = q.D % (16 / sz) == 0 && aligned16(q.h_init) && aligned16(q.dh_last) && aligned16(q.h_last) &&
+                       rows16(q.x, sz) && rows16(q.g, sz) && rows16(q.h, sz) && rows16(q.dx, sz) && rows16(q.dg, sz);
   for (const ScanSeq *t : {&q.x, &q.g, &q.h, &q.dx, &q.dg})
     if (t->ts >= (1LL << 29))
       return fail(SNNB_ERR_UNSUPPORTED, "gated_scan: time strides of 2^29 values or more are not implemented");
