@@ -325,3 +325,15 @@ def test_rows_behind_the_last_add_nothing_to_the_parameters(M, D, row):
         assert float(got[3]) == q * float(w[3].float().sign())
         got[3] = 0
         assert bool(torch.isfinite(got).all())
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 5, 37])
+@pytest.mark.parametrize("D", [8, 63, 64, 128, 200, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_eps_zero_with_groups_that_have_no_row(M, D, dtype):
+    """Narrow rows share a block, and with these row counts some of its groups have none: with eps = 0 the norm of such a row
+    is infinite, which must not reach the parameters' gradients. No row is zero, so every value is defined."""
+    for post, pre, has_dz in ((True, True, True), (True, True, False), (False, True, True), (True, False, False)):
+        _, r = _check(M, D, dtype, post=post, pre=pre, has_dz=has_dz, eps=0.0, seed=M + D)
+        assert all(bool(torch.isfinite(t).all()) for t in r if t is not None)

@@ -355,13 +355,8 @@ __global__ void __launch_bounds__(TPR > 0 ? TPR : 128, MINB) block_norm_backward
   auto to_stage = [&](int st) {
     if constexpr (ST > 0) { y.p = slots + st * 5 * SLOT; g.p = y.p + SLOT; r.p = g.p + SLOT; o.p = r.p + SLOT; z.p = o.p + SLOT; }
   };
-  // a row that does not exist adds nothing to the column sums: all of it is zero, for infinities of the row before it
-  // would make NaN of zeros
   auto fetch = [&](int64_t row) {
-    if (row >= q.M) {
-      y.clear(); g.clear(); r.clear(); o.clear(); z.clear();
-      return;
-    }
+    if (row >= q.M) return;
     y.template load<ALL>(yp, stride * q.ys, step, in);
     g.template load<ALL>(gp, stride * q.gs, step, in);
     r.template load<ALL>(rp, stride * q.rs, step, in);
@@ -382,6 +377,8 @@ __global__ void __launch_bounds__(TPR > 0 ? TPR : 128, MINB) block_norm_backward
   int st = 0;
   const float inv_d = 1.f / (float)q.D;
   for (int64_t first = (int64_t)blockIdx.x * groups; first < q.M; first += stride, m += stride, at += stride * q.D) {
+    // A group that has no row left works on whatever is in its place, and neither stores nor adds any of it: even a row of
+    // zeros would add 0 * rstd(0) to the column sums, which is not a number where eps is zero.
     const bool live = TPR > 0 || m < q.M;
     if constexpr (ST > 0) {
       to_stage(st == 0 ? ST - 1 : st - 1);
@@ -450,7 +447,7 @@ __global__ void __launch_bounds__(TPR > 0 ? TPR : 128, MINB) block_norm_backward
         z.get(v, f);
         v_mul(f, ro, f);
         if constexpr (ACC_SH) add(acc_sh + q.D, v, f, G[v]);
-        else v_fma(f, G[v], aw[v], aw[v]);
+        else if (live) v_fma(f, G[v], aw[v], aw[v]);
         o.get(v, t);
         v_fma(mo, G[v], t, G[v]);
         param_at(1, v, p);
@@ -466,7 +463,7 @@ __global__ void __launch_bounds__(TPR > 0 ? TPR : 128, MINB) block_norm_backward
         param_at(0, v, p);
         v_fma(t, p, acc, acc);
         if constexpr (ACC_SH) add(acc_sh, v, t, al);
-        else v_fma(t, al, aq[v], aq[v]);
+        else if (live) v_fma(t, al, aq[v], aq[v]);
       }
     }
     float me[VEC];
