@@ -82,8 +82,8 @@ int snnb_version(void);
 /* Text of the last error raised on the calling thread ("" if none). */
 const char *snnb_last_error(void);
 
-/* Reads and clears the device-side status word that the tcgen05 kernels set
- * when one of their bounded mbarrier waits gives up. Synchronises the device.
+/* Reads and clears the device-side status word that the tcgen05 kernels and the
+ * gated scan set when one of their bounded mbarrier waits gives up. Synchronises the device.
  * 0 = no kernel reported a problem. Diagnostic only; never called on the hot
  * path. */
 int snnb_device_status(int *status_out);
@@ -94,9 +94,11 @@ int snnb_device_status(int *status_out);
  * that runs on the timestep-pair, split or 1x1 kernel: its waits give up after `limit_cycles` SM cycles (1e3 .. 4e9)
  * instead of about two seconds, and its first thread block announces one operand tile that it never loads. That block's
  * waits therefore run out: it records the fact in the status word, releases its tensor memory and returns,
- * while the other blocks finish normally. Nothing traps, faults or hangs; the armed call returns SNNB_OK, its
- * output is incomplete, and snnb_device_status() then reports a non-zero status once. The call after it runs
- * normally again.
+ * while the other blocks finish normally. A snnb_gated_scan or snnb_gated_scan_backward call that splits its sequences
+ * over clusters of blocks is armed as well: there the last block of the first cluster waits in its first step for a map
+ * that nobody sends, and the blocks of that cluster give up one after the other. Nothing traps, faults or hangs; the
+ * armed call returns SNNB_OK, its output is incomplete, and snnb_device_status() then reports a non-zero status once.
+ * The call after it runs normally again.
  */
 int snnb_selftest_arm_wait_timeout(long long limit_cycles);
 

@@ -85,7 +85,8 @@ int conv_split_plan(const ConvArgs &a);
 int conv_split(const ConvArgs &a, int S, cudaStream_t stream);
 int split_device_status(int *out);
 // Self-test of the bounded waits (snnb_selftest_arm_wait_timeout): if armed, hands the shortened limit and the
-// "drop one load" switch to the next launch of the timestep-pair, split or 1x1 kernel and disarms.
+// "drop one load" switch to the next launch of the timestep-pair, split or 1x1 kernel, or of a gated scan over
+// clusters, and disarms.
 void consume_wait_selftest(long long *limit_cycles, int *drop_load);
 
 // GEMM + LIF stage of the 7x7 / stride 2 stem on the re-laid image (stem.cu): persistent tcgen05 kernel

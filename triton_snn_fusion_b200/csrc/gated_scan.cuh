@@ -20,8 +20,13 @@ struct ScanArgs {
   const int *lengths;
   int64_t T, B, D;
   int state_f32, leaky;
-  int tiles_d;        // channel tiles of a row; filled in by the launch
+  // filled in by the launch
+  int tiles_d;            // channel tiles of a row
+  long long wait_limit;   // bound of every wait of a cluster's exchange, in SM cycles (about two seconds unless a self-test shortens it)
+  int miss_map;           // self-test: the last block of the first cluster waits for a map that nobody sends
 };
+
+void consume_wait_selftest(long long *limit_cycles, int *drop_load);      // conv_pair.cu
 
 // One translation unit per activation type. gate_kind as in the C ABI; aligned: every row starts on a 16-byte boundary
 // and ends on one, and so do the states.

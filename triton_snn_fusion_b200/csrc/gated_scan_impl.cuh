@@ -119,13 +119,16 @@ static __device__ int g_scan_status = 0;      // set when a bounded wait gave up
 // barrier. (A cluster barrier instead would order all stores of h before it as well: with it, two blocks that shared a
 // sequence took longer than one alone.) Two slots: a block sends for step i + 2 after it has received everybody's map of
 // step i + 1, which they sent after they had read those of step i.
+// A block of which a joiner's wait gives up (the maps of a step did not come within about two seconds) sends, re-arms and
+// reads nothing from its next step on, so the others' waits run out as well, and the call's results are worthless. No block
+// leaves before all of its cluster have stopped sending, for a map may still be on its way to one that has given up.
 template <int CH> struct Exchange {
   float2 *map;            // [2][S][CH]
   uint32_t bar, bytes;    // two barriers, 8 bytes apart
   int S, rank;
-  int *abort;
+  volatile int *abort;    // a wait of the block gave up; in shared memory, for the backward pass has no register for it
 
-  __device__ __forceinline__ void init(float2 *m, uint64_t *bars, int *abort_flag, int s, int r) {
+  __device__ __forceinline__ void init(float2 *m, uint64_t *bars, int *abort_flag, int s, int r, const ScanArgs &q) {
     map = m; bar = umma::smem_u32(bars); S = s; rank = r; abort = abort_flag;
     bytes = (uint32_t)(S * CH * sizeof(float2));
     if (S == 1) return;
@@ -134,13 +137,14 @@ template <int CH> struct Exchange {
       umma::mbar_init(bar, 1);
       umma::mbar_init(bar + 8, 1);
       umma::fence_mbar_init();
-      umma::mbar_expect_tx(bar, bytes);
+      umma::mbar_expect_tx(bar, bytes + (q.miss_map && (int)blockIdx.x == S - 1 ? 8 : 0));
       umma::mbar_expect_tx(bar + 8, bytes);
     }
     cg::this_cluster().sync();
   }
-  // threads 0 .. CH - 1, one channel each
-  __device__ __forceinline__ void swap(int it, float A, float X) {
+  // threads 0 .. CH - 1, one channel each; false: there are no maps
+  __device__ __forceinline__ bool swap(const ScanArgs &q, int it, float A, float X) {
+    if (*abort) return false;
     const int slot = it & 1;
     const uint32_t at = umma::smem_u32(map + (slot * S + rank) * CH + threadIdx.x), b = bar + 8 * slot;
     for (int r = 0; r < S; ++r) {
@@ -150,8 +154,20 @@ template <int CH> struct Exchange {
       asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];"
                    ::"r"(ra), "f"(A), "f"(X), "r"(rb) : "memory");
     }
-    if (!umma::mbar_wait(b, (it >> 1) & 1, abort)) atomicExch(&g_scan_status, 1);
+    if (!umma::mbar_wait(b, (it >> 1) & 1, abort, q.wait_limit)) {
+      atomicExch(&g_scan_status, 1);
+      return false;
+    }
     if (threadIdx.x == 0) umma::mbar_expect_tx(b, bytes);      // for step it + 2
+    return true;
+  }
+  // all threads, at the end of the kernel; nothing has to be ordered, so the barrier does not wait for the stores of h
+  __device__ __forceinline__ void leave() const {
+    if (S == 1) return;
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+    asm volatile("barrier.cluster.wait;" ::: "memory");
+    if (*abort)      // the last maps of the others land meanwhile
+      for (int i = 0; i < 32; ++i) __nanosleep(1000);
   }
   __device__ __forceinline__ float2 of(int it, int r) const { return map[((it & 1) * S + r) * CH + threadIdx.x]; }
 };
@@ -284,7 +300,7 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_kernel(const __gr
   for (int i = 0; i < STAGES - 1; ++i) fetch((i * S + g.rank) * TC, i);
   Exchange<CH> cluster_maps;
   if constexpr (SEG > 1)      // behind every block's read of h_init: the first block may write h_last to the same buffer
-    cluster_maps.init(reinterpret_cast<float2 *>(dyn + (STAGED ? STAGES * G::STAGE : 0)), bars, &abort_flag, S, g.rank);
+    cluster_maps.init(reinterpret_cast<float2 *>(dyn + (STAGED ? STAGES * G::STAGE : 0)), bars, &abort_flag, S, g.rank, q);
   int st = 0, base = 0, it = 0;
   // One tile. FULL: every step of it counts and all channels exist, so nothing is asked.
   auto work = [&](auto full) {
@@ -353,14 +369,15 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_kernel(const __gr
             tH = fmaf(fA, tH, sH[s * CH + threadIdx.x]);
             tA *= fA;
           }
-          cluster_maps.swap(it, tA, tH);
-          float c = carry[0];
-          for (int r = 0; r < S; ++r) {
-            if (r == g.rank) h1 = c;
-            const float2 m = cluster_maps.of(it, r);
-            c = fmaf(m.x, c, m.y);
+          if (cluster_maps.swap(q, it, tA, tH)) {
+            float c = carry[0];
+            for (int r = 0; r < S; ++r) {
+              if (r == g.rank) h1 = c;
+              const float2 m = cluster_maps.of(it, r);
+              c = fmaf(m.x, c, m.y);
+            }
+            carry[0] = c;
           }
-          carry[0] = c;
         }
         if (jok && q.ckpt && tile0 > 0 && tile0 % kCkpt == 0 && tile0 < T_)
           q.ckpt[(int64_t)(tile0 / kCkpt - 1) * q.B * q.D + ji] = h1;
@@ -389,8 +406,10 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_kernel(const __gr
     else work(std::false_type{});
   }
   if (g.rank == 0) state_store<T, CV>(q.h_last, q.state_f32, ji, jok, carry);
-  if constexpr (SEG > 1)      // tiles behind the sequence
-    for (; base < T_; base += S * TC) g.zero(q.h, base + g.rank * TC);
+  if constexpr (SEG > 1) {
+    for (; base < T_; base += S * TC) g.zero(q.h, base + g.rank * TC);      // tiles behind the sequence
+    cluster_maps.leave();
+  }
 }
 
 // The same split from the end. With c the gradient that reaches a step from the one behind it (c = a_{t+1} lam_{t+1}):
@@ -446,7 +465,7 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_backward_kernel(c
   Exchange<CH> cluster_maps;
   if constexpr (SEG > 1) {
     // behind every block's read of dh_last: the first block may write dh_init to the same buffer
-    cluster_maps.init(reinterpret_cast<float2 *>(dyn + (STAGED ? STAGES * G::STAGE : 0)), bars, &abort_flag, S, g.rank);
+    cluster_maps.init(reinterpret_cast<float2 *>(dyn + (STAGED ? STAGES * G::STAGE : 0)), bars, &abort_flag, S, g.rank, q);
     for (int t = last; t > base && t >= 0; t -= S * TC) {      // tiles behind the sequence
       g.zero(q.dx, t + g.rank * TC);
       g.zero(q.dg, t + g.rank * TC);
@@ -535,14 +554,15 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_backward_kernel(c
             tC = fmaf(fA, tC, sC[s * CH + jc]);
             tA *= fA;
           }
-          cluster_maps.swap(it, tA, tC);
-          float v = carry[0];
-          for (int r = S - 1; r >= 0; --r) {
-            if (r == g.rank) c1 = v;
-            const float2 mp = cluster_maps.of(it, r);
-            v = fmaf(mp.x, v, mp.y);
+          if (cluster_maps.swap(q, it, tA, tC)) {
+            float v = carry[0];
+            for (int r = S - 1; r >= 0; --r) {
+              if (r == g.rank) c1 = v;
+              const float2 mp = cluster_maps.of(it, r);
+              v = fmaf(mp.x, v, mp.y);
+            }
+            carry[0] = v;
           }
-          carry[0] = v;
         }
         c1 = join<SEG, -1>(sA + jc, sC + jc, CH, c1);
         if (S == 1) carry[0] = c1;
@@ -629,6 +649,7 @@ __global__ void __launch_bounds__(LANES *SEG, MINB) gated_scan_backward_kernel(c
     else work(std::false_type{});
   }
   if (g.rank == 0) state_store<T, CV>(q.h_last, q.state_f32, ji, jok && join_c, carry);
+  if constexpr (SEG > 1) cluster_maps.leave();
 }
 
 // smem: of the stages; the exchange of a cluster of S comes on top.
@@ -637,6 +658,9 @@ int launch_tiles(ScanArgs q, int threads, int CH, int S, int smem, cudaStream_t 
   const int64_t tiles_d = (q.D + CH - 1) / CH, blocks = tiles_d * q.B * S;
   if (blocks > 0x7fffffffLL) return fail(SNNB_ERR_INVALID, "gated_scan: problem too large");
   q.tiles_d = (int)tiles_d;
+  q.wait_limit = 4000000000ll;
+  q.miss_map = 0;
+  if (S > 1) consume_wait_selftest(&q.wait_limit, &q.miss_map);
   cudaError_t e = smem > 0 ? raise_smem_limit_once<Kern>(smem + 2 * kMaxCluster * CH * 8) : cudaSuccess;
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
