@@ -683,14 +683,26 @@ int launch_tiles(ScanArgs q, int threads, int CH, int S, int smem, cudaStream_t 
   return SNNB_OK;
 }
 
-// Blocks of a cluster for `tiles` channel tiles of `steps` tiles of time: doubled while all blocks still run at once, four
-// to an SM, and each has a tile of time. Measured (bf16, us, forward / backward) with 1, 2, 4, 8 blocks: B1 T4096 D2048
-// (64 tiles) 45 31 22 20 / 84 53 37 41; B4 T2048 D2048 (256) 33 31 33 37 / 57 51 59 63; B16 T1024 D1024 (512)
-// 28 32 36 43 / 48 51 57 73; B1 T100 D4096 (one tile of time) 7.6 7.7 9.5 12.3 / 9.5 9.5 15.8 21.8.
-int scan_cluster(int64_t tiles, int64_t steps) {
+// Blocks of a cluster for `tiles` channel tiles of `steps` tiles of time: doubled while each block has a tile of time and
+// all blocks run at once, `most` of them to an SM, or fewer where shared memory (`smem` bytes a block, and the exchange of
+// the cluster's CH channels) holds fewer: the backward pass of 16-bit rows, with 55 KB, has room for four blocks in clusters
+// of one or two and for three in larger ones. Device time (bf16, us, forward / backward) with 1, 2, 4, 8 blocks:
+//   B1 T4096 D2048 (64 tiles)       33 23 16 14 / 61 39 26 31       B1 T16384 D2048   126 85 56 45 / 238 148 95 106
+//   B2 T4096 D2048 (128)            34 29 24 27 / 62 49 52 51       B1 T1024 D4096    10.3 10.1 8.9 11.2 / 17 15 17 18
+//   B4 T2048 D2048 (256)            24 23 25 29 / 42 40 48 55       B16 T1024 D1024 (512)   21 25 28 37 / 37 40 49 64
+//   B2 T16384 D512 (32)             126 85 44 31 / 238 147 75 50
+// The ragged backward kernel (512 threads, two blocks an SM) is given as many blocks as two rounds take, its loads being
+// what it waits for: B2 T4096 D2047 (128 tiles) 188 131 110 105, B1 T8192 D2047 (64) 361 203 131 116, B4 T2048 D2047 (256)
+// 120 105 100 107; at short sequences one round is a little better: B1 T1024 D2047 38 23 17 18, B6 T1031 D1001 fp32 (192)
+// 51 53 55 75.
+int scan_cluster(int64_t tiles, int64_t steps, int CH, int most, int smem) {
   const int sms = sm_count() > 0 ? sm_count() : 148;
+  auto at_once = [&](int S) {
+    const int room = 228 * 1024 / (smem + 2 * S * CH * 8 + 64 + 1024);      // the barriers, and what the system takes of each block
+    return (int64_t)sms * (room < most ? room : most);
+  };
   int S = 1;
-  while (S < kMaxCluster && 2 * S <= steps && 2 * S * tiles <= 4 * sms) S *= 2;
+  while (S < kMaxCluster && 2 * S <= steps && 2 * S * tiles <= at_once(2 * S)) S *= 2;
   return S;
 }
 
@@ -735,7 +747,8 @@ template <typename T, bool SIG, Rows R> int forward(const ScanArgs &q, cudaStrea
   constexpr bool RAG = R == Rows::ragged;
   constexpr int V = RAG ? 2 : VEC, LANES = RAG ? 16 : 8, SEG = 16, L = RAG ? 4 : 8, ST = RAG ? 0 : 2, MINB = 4;
   using G = Tile<T, R, V, LANES, SEG, L, ST, 2>;
-  const int S = scan_cluster((q.D + G::CH - 1) / G::CH * q.B, (q.T + G::TC - 1) / G::TC);
+  const int S = scan_cluster((q.D + G::CH - 1) / G::CH * q.B, (q.T + G::TC - 1) / G::TC, G::CH, 4,
+                             ST * G::STAGE + 2 * SEG * G::CH * 4);
   if (q.leaky)
     return launch_tiles<gated_scan_kernel<T, R, SIG, 1, V, LANES, SEG, L, ST, MINB>>(q, LANES * SEG, G::CH, S, ST * G::STAGE, s);
   return launch_tiles<gated_scan_kernel<T, R, SIG, 0, V, LANES, SEG, L, ST, MINB>>(q, LANES * SEG, G::CH, S, ST * G::STAGE, s);
@@ -756,7 +769,8 @@ template <typename T, bool SIG, Rows R> int backward(const ScanArgs &q, cudaStre
   constexpr bool RAG = R == Rows::ragged;
   constexpr int V = RAG ? 2 : VEC, LANES = RAG ? 16 : 8, SEG = RAG ? 32 : 16, L = RAG ? 4 : 8, ST = RAG ? 0 : 2, MINB = RAG ? 2 : 4;
   using G = Tile<T, R, V, LANES, SEG, L, ST, 3>;
-  const int S = scan_cluster((q.D + G::CH - 1) / G::CH * q.B, (q.T + G::TC - 1) / G::TC);
+  const int S = scan_cluster((q.D + G::CH - 1) / G::CH * q.B, (q.T + G::TC - 1) / G::TC, G::CH, 4,
+                             ST * G::STAGE + 3 * SEG * G::CH * 4);
   if (q.leaky)
     return launch_tiles<gated_scan_backward_kernel<T, R, SIG, 1, V, LANES, SEG, L, ST, MINB>>(q, LANES * SEG, G::CH, S, ST * G::STAGE, s);
   return launch_tiles<gated_scan_backward_kernel<T, R, SIG, 0, V, LANES, SEG, L, ST, MINB>>(q, LANES * SEG, G::CH, S, ST * G::STAGE, s);
