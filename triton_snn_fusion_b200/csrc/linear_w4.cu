@@ -12,12 +12,10 @@
 // its row, so that the four lanes of a row cover one group and its loads are 16, 8 or 4 bytes wide, and the matching x
 // values, eight neighbours at a time.
 //
-// What bounds it, on B200: not the bytes. 1 token, bf16: 4096 -> 4096 12 us (8.4 MB, 1.3 us at the copy rate, 3 of them the
-// launch), 8192 -> 16384 27 us = 2.5 TB/s (38 % of the copy rate); 16 tokens 41 us. With the weights in L2 it is as slow. A
-// warp spends 160 to 230 instructions on the 2048 weights of a step and tile where 88 unpack them, at 0.5 instructions a
-// cycle. Tried and no faster: weights through a ring of asynchronous copies, rows instead of K split over the warps with a
-// cluster joining K, x in registers or permuted in shared memory, several sums a group, loads without branches.
-// Three blocks an SM in place of two (80 registers) take 55 us for 16 tokens of 8192 -> 16384 and 35 for one.
+// What bounds it, on B200: not the bytes. Device time, bf16: 1 token 4096 -> 4096 5.6 us (8.4 MB, 1.3 us at the copy rate),
+// 8192 -> 16384 21 us = 3.3 TB/s (50 % of the copy rate); 16 tokens 38 us with zero points, 36 without. A warp spends 160
+// to 230 instructions on the 2048 weights of a step and tile where 88 unpack them, at 0.5 instructions a cycle. Three blocks
+// an SM in place of two (80 registers) took 55 us for 16 tokens of 8192 -> 16384 and 35 for one.
 #include "common.cuh"
 
 #include <type_traits>
@@ -361,18 +359,26 @@ template <typename T, bool ZERO, int G, int NT, int RT, int DEPTH> int go(const 
   return SNNB_OK;
 }
 
-// Rows a warp and steps ahead, measured on B200 in us for (RT, DEPTH) = (1, 4) (2, 2) (2, 1) (4, 1), groups of 128, bf16:
-//   1 token    4096 -> 4096 12.3 12.3 12.3 14.3, fp32 12.3 14.3 14.3 16.4; 8192 -> 16384 34.8 30.8 30.7 26.7
-//   8 tokens   8192 -> 8192 28.7 20.5 20.5 22.5
-//   16 tokens  8192 -> 16384 - 43.0 41.0 43.0; 4096 -> 4096 - 14.3 12.3 18.4
-//   32 tokens  8192 -> 8192 - 43.0 45.1 32.8; 64 tokens 4096 -> 8192 - 47.1 47.1 34.8
-// More rows a warp share what a step costs beside the weights; fewer blocks than twice the SMs cost more than that.
+// Rows a warp and steps ahead: device time on B200 in us for (RT, DEPTH) = (1, 4) (2, 2) (2, 1) (4, 1), groups of 128, bf16;
+// in brackets the tiles of 16 rows.
+//   1 token    4096 -> 2368 (148)   4.2  5.9  6.2  8.2      4096 -> 12288 (768)   12.4 12.7 10.2 11.6
+//              4096 -> 4096 (256)   5.6  6.3  6.4  8.5      4096 -> 13312 (832)   12.7 12.8 10.3 11.7
+//              4096 -> 4736 (296)   5.7  6.5  6.6  8.6      4096 -> 14336 (896)   14.6 14.2 13.7 11.8
+//              4096 -> 5120 (320)   7.2  7.4  7.3  8.7      4096 -> 16384 (1024)  14.9 14.7 14.1 11.9
+//              4096 -> 8192 (512)   9.8  8.3  8.1  9.6      8192 -> 16384 (1024)  28.7 24.8 24.5 21.0
+//   fp32       4096 -> 4096 (256)   7.6  8.0  8.1 10.1      4096 -> 16384 (1024)  23.8 17.5 17.6 14.0
+//   8 tokens   8192 -> 8192 (512)  21.5 15.2 15.3 16.7      4096 -> 12288 (768)   16.3 14.2 12.6 13.7
+//   16 tokens  4096 -> 4096 (256)   9.2  7.9  8.3 10.8      8192 -> 16384 (1024)  50.3 35.7 35.7 36.8
+// and with (RT, DEPTH) = (2, 2) (2, 1) (4, 1), 32 tokens 8192 -> 8192 37 38 27, 64 tokens 4096 -> 8192 40 41 29.
+// More rows a warp share what a step costs beside the weights; fewer blocks than twice the SMs cost more than that. With two
+// tiles a block three blocks run on an SM (65 registers; 111 and two blocks with two steps ahead), so that up to six tiles an
+// SM are one round.
 template <typename T, bool ZERO, int G> int by_tokens(const W4Args &a, cudaStream_t s) {
   const int cols = (int)(a.M < 64 ? a.M : 64) * kPieces<T>, tiles = (a.N + 15) / 16, sms = sm_count() > 0 ? sm_count() : 148;
   if (cols > 16) return go<T, ZERO, G, 4, 4, 1>(a, s);
   if (cols > 8) return go<T, ZERO, G, 2, 2, 1>(a, s);
   if (tiles <= 2 * sms) return go<T, ZERO, G, 1, 1, 4>(a, s);
-  if (tiles < 6 * sms) return go<T, ZERO, G, 1, 2, 2>(a, s);
+  if (tiles < 6 * sms) return go<T, ZERO, G, 1, 2, 1>(a, s);
   return go<T, ZERO, G, 1, 4, 1>(a, s);
 }
 
