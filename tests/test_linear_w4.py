@@ -216,3 +216,27 @@ def test_infinite_tokens(dtype, M):
         weight = (q[:, k // 2] >> (4 * (k % 2)) & 15).double() - z[:, k // G].double()
         want = weight * v
         assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.nan_to_num(nan=0.0, posinf=2, neginf=-2), want.nan_to_num(nan=0.0, posinf=2, neginf=-2))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [1, 12, 40])
+def test_large_zero_points(dtype, M):
+    """Zero points up to 127 are numbers like any other, in each type. A larger one is outside what is documented: fp16 still
+    has its value, the other types have no number for it and answer NaN in its rows alone."""
+    K, N, G = 256, 70, 64
+    x, q, s, _, b = _inputs(M, K, N, G, dtype)
+    zs = torch.tensor([0, 15, 16, 63, 64, 100, 126, 127], dtype=torch.uint8)
+    z = zs[(torch.arange(N)[:, None] + 3 * torch.arange(K // G)) % 8].contiguous()
+    ref, err = orc.linear_w4(x, q, s, z, b, G)
+    y = ops.run_linear_w4(_dev(x), _dev(q), _dev(s), _dev(z), _dev(b), group_size=G)
+    orc.assert_within(y, ref, err)
+    z[5, 1], z[40, 3] = 128, 255
+    ref, err = orc.linear_w4(x, q, s, z, b, G)
+    y2 = ops.run_linear_w4(_dev(x), _dev(q), _dev(s), _dev(z), _dev(b), group_size=G)
+    if dtype == torch.float16:
+        orc.assert_within(y2, ref, err)
+    else:
+        assert bool(y2[:, [5, 40]].isnan().all())
+        keep = [n for n in range(N) if n not in (5, 40)]
+        assert torch.equal(y2[:, keep], y[:, keep])

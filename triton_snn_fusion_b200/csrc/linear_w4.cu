@@ -65,9 +65,10 @@ template <typename H> __device__ __forceinline__ void unpack8(uint32_t w, const 
     for (int i = 0; i < 4; ++i) p[i] = minus<H>(and_or(w >> (4 * i), 0x000f000fu, magic<H>()), zero[0]);
   }
 }
-// the two constants of unpack8 for a zero point of at most 127
+// The two constants of unpack8 for a zero point. Beyond 127, magic + zero is no bf16 number any more: that makes the weights
+// NaN rather than wrong.
 template <typename H> __device__ __forceinline__ void zeros_of(uint32_t z, uint32_t (&zero)[2]) {
-  zero[0] = magic<H>() + 0x00010001u * z;
+  zero[0] = !std::is_same_v<H, __half> && z > 127 ? 0x7fff7fffu : magic<H>() + 0x00010001u * z;
   if constexpr (std::is_same_v<H, __half>) {      // -(64 + z): 64 .. 127 have steps of 1/16 in fp16, beyond that of 1/8
     const __half2 v = __half2half2(__int2half_rn(-64 - (int)z));
     zero[1] = *reinterpret_cast<const uint32_t *>(&v);

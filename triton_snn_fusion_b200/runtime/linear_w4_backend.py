@@ -21,7 +21,7 @@ GROUP_SIZES = (32, 64, 128)
 class W4Weight(NamedTuple):
     q_weight: torch.Tensor              # [N, K // 2] uint8, weight k in the low (k even) or high half of byte k // 2
     scales: torch.Tensor                # [N, ceil(K / G)]
-    zeros: Optional[torch.Tensor]       # [N, ceil(K / G)] uint8 (at most 127), None = 8
+    zeros: Optional[torch.Tensor]       # [N, ceil(K / G)] uint8 (at most 127, see run_linear_w4), None = 8
 
 
 def quantize_linear_w4(weight: torch.Tensor, group_size: int = 128, symmetric: bool = True) -> W4Weight:
@@ -119,7 +119,8 @@ def run_linear_w4(
     verbose: bool = False,
 ) -> torch.Tensor:
     """x [..., K] -> [..., N] in x's dtype. ``q_weight``, ``scales`` and ``zeros`` as ``quantize_linear_w4`` lays them out;
-    keep them contiguous (they are copied at every call otherwise). ``out``: a contiguous tensor to write into, apart from x."""
+    keep them contiguous (they are copied at every call otherwise). A zero point above 127, which no 4-bit weight needs, makes
+    its output NaN for bf16 and fp32 tokens. ``out``: a contiguous tensor to write into, apart from x."""
     if not _is_plain(x, q_weight, scales, zeros, bias, group_size):
         raise_reasons("linear_w4", check_linear_w4_support(x, q_weight, scales, zeros, bias, group_size), False, verbose)
     K, N = int(x.shape[-1]), int(q_weight.shape[0])
