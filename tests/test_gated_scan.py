@@ -368,3 +368,15 @@ def test_output_refusals_on_the_device():
         ops.run_temporal_gated_scan(x, x, h_last_out=torch.zeros(2, 8, device=DEV).half())
     with pytest.raises(RuntimeError, match="overlap"):
         ops.run_temporal_gated_scan(x, x, h_seq_out=torch.zeros(1, 2, 8, device=DEV).expand(4, 2, 8))
+
+
+def test_states_that_are_no_tensors_are_refused():
+    """A carried state is a tensor, a 0-dim tensor or None; anything else was once taken for zeros without a word."""
+    x = torch.zeros(4, 2, 8)
+    for bad in (1.0, [[0.0] * 8] * 2, "zeros"):
+        with pytest.raises(RuntimeError, match="h_init is"):
+            ops.run_temporal_gated_scan(x, x, bad)
+        with pytest.raises(RuntimeError, match="h_init is"):
+            ops.run_temporal_gated_scan_backward(x, x, x, bad)
+        with pytest.raises(RuntimeError, match="dh_last is"):
+            ops.run_temporal_gated_scan_backward(x, x, x, dh_last=bad)

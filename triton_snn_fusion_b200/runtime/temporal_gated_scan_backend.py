@@ -47,6 +47,13 @@ def _like(g: Gate, name: str, t, shape, dtype=None) -> None:
         g.add("unsupported_dtype", f"{name} is {t.dtype} on {t.device}, expected {dtype or g.lead.dtype} on {g.lead.device}")
 
 
+def _state(g: Gate, name: str, t):
+    """A carried state, None where the call starts from zeros."""
+    if t is not None and not isinstance(t, torch.Tensor):
+        g.add("", f"{name} is {type(t).__name__}, expected a Tensor (0-dim or None for zeros)")
+    return state_or_none(t)
+
+
 def check_temporal_gated_scan_support(x_seq, gate_seq, h_init, gate, lengths=None, batch_first=False,
                                       state_dtype=None) -> List[str]:
     """Reasons why the scan cannot take this call (empty = it can)."""
@@ -61,7 +68,7 @@ def check_temporal_gated_scan_support(x_seq, gate_seq, h_init, gate, lengths=Non
         _, B, D = _sizes(x_seq, batch_first)
         if state_dtype is not None and state_dtype not in (x_seq.dtype, torch.float32):
             g.add("unsupported_dtype", f"state_dtype is {state_dtype}, the state is {x_seq.dtype} or torch.float32")
-        h0 = state_or_none(h_init)
+        h0 = _state(g, "h_init", h_init)
         if h0 is not None:
             _like(g, "h_init", h0, (B, D), h0.dtype)
             if h0.dtype not in (x_seq.dtype, torch.float32) or state_dtype not in (None, h0.dtype):
@@ -167,7 +174,7 @@ def _check_backward(dh_seq, x_seq, gate_seq, h_init, ckpt, dh_last, gate, length
         T, B, D = _sizes(x_seq, batch_first)
         g = Gate("x_seq", x_seq)
         _like(g, "dh_seq", dh_seq, x_seq.shape)
-        h0, dl = state_or_none(h_init), state_or_none(dh_last)
+        h0, dl = state_or_none(h_init), _state(g, "dh_last", dh_last)
         if dl is not None:
             _like(g, "dh_last", dl, (B, D), h0.dtype if h0 is not None else dl.dtype)
             if dl.dtype not in (x_seq.dtype, torch.float32):
