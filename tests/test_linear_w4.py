@@ -240,3 +240,24 @@ def test_large_zero_points(dtype, M):
         assert bool(y2[:, [5, 40]].isnan().all())
         keep = [n for n in range(N) if n not in (5, 40)]
         assert torch.equal(y2[:, keep], y[:, keep])
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 6e-7), (torch.float16, 2e-7), (torch.float16, 4e-6), (torch.float16, 6e4),
+                                        (torch.bfloat16, 3e38), (torch.float32, 3e38), (torch.float32, 1e-44)])
+def test_quantized_weights_at_the_ends_of_the_types(symmetric, dtype, size):
+    """Groups so small that their scale is a subnormal number, which rounds by up to half of itself, and groups as wide as the
+    type: each weight within half a step of what it is read back as (a whole one with a rounded zero point; 2^-8 of the widest
+    weight, 15 steps, for the scale's rounding), and the step no wider than a seventh (fifteenth) of the group or the type's
+    smallest number, whichever is more, up to that rounding."""
+    G = 32
+    w = ((torch.rand(6, 64, generator=torch.Generator().manual_seed(1)) * 2 - 1) * size).to(dtype)
+    r = ops.quantize_linear_w4(w, G, symmetric)
+    assert bool(torch.isfinite(r.scales).all())
+    step = r.scales.double()[:, torch.arange(64) // G]
+    back = orc.unpack_w4(r.q_weight, r.scales, r.zeros, G)
+    assert bool(((back - w.double()).abs() <= step * ((0.5 if symmetric else 1.0) + 15 * 2.0 ** -8)).all())
+    g = w.double().view(6, 2, G)
+    exact = g.abs().amax(-1) / 7 if symmetric else (g.amax(-1).clamp(min=0) - g.amin(-1).clamp(max=0)) / 15
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    assert bool((r.scales.double() <= exact * (1 + 2.0 ** -8) + tiny).all())

@@ -34,14 +34,19 @@ def quantize_linear_w4(weight: torch.Tensor, group_size: int = 128, symmetric: b
         raise RuntimeError(f"unsupported_shape: K = {K} (a multiple of 32), groups of {group_size} (one of {GROUP_SIZES})")
     groups = -(-K // group_size)
     w = torch.nn.functional.pad(weight.float(), (0, groups * group_size - K)).view(N, groups, group_size)
+    largest = w.abs().amax(-1)
     if symmetric:
-        scale = w.abs().amax(-1) / 7
-        zero = torch.full_like(scale, 8.0)
+        exact = largest / 7
+        zero = torch.full_like(exact, 8.0)
     else:
         lo, hi = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
-        scale = (hi - lo) / 15
+        exact = torch.where((hi - lo).isinf(), hi / 15 - lo / 15, (hi - lo) / 15)
         zero = None
-    scale = scale.to(weight.dtype)
+    scale = exact.to(weight.dtype)
+    # a subnormal scale may have lost up to all of itself to rounding: the next larger one then
+    lost = (scale.float() < exact * (1 - 2.0 ** -7)) | ((scale == 0) & (largest > 0))
+    smallest = torch.finfo(weight.dtype).tiny * torch.finfo(weight.dtype).eps
+    scale = torch.where(lost, (scale.float() + smallest).to(weight.dtype), scale)
     scale = torch.where(scale == 0, torch.ones_like(scale), scale)
     if zero is None:
         zero = (-lo / scale.float()).round().clamp(0, 15)
