@@ -261,3 +261,15 @@ def test_quantized_weights_at_the_ends_of_the_types(symmetric, dtype, size):
     exact = g.abs().amax(-1) / 7 if symmetric else (g.amax(-1).clamp(min=0) - g.amin(-1).clamp(max=0)) / 15
     tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
     assert bool((r.scales.double() <= exact * (1 + 2.0 ** -8) + tiny).all())
+
+
+def test_quantizing_a_parameter_keeps_no_graph():
+    """The 4-bit weights of a model's parameter are plain tensors: they must not hold the full weight through autograd."""
+    w = torch.nn.Parameter(torch.randn(8, 64, generator=torch.Generator().manual_seed(0)))
+    for symmetric in (True, False):
+        r = ops.quantize_linear_w4(w, 32, symmetric)
+        plain = ops.quantize_linear_w4(w.detach(), 32, symmetric)
+        for a, b in zip(r, plain):
+            assert (a is None) == (b is None)
+            if a is not None:
+                assert not a.requires_grad and a.grad_fn is None and torch.equal(a, b)

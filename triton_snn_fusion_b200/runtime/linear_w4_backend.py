@@ -33,7 +33,7 @@ def quantize_linear_w4(weight: torch.Tensor, group_size: int = 128, symmetric: b
     if group_size not in GROUP_SIZES or K % 32 != 0 or K == 0:
         raise RuntimeError(f"unsupported_shape: K = {K} (a multiple of 32), groups of {group_size} (one of {GROUP_SIZES})")
     groups = -(-K // group_size)
-    w = torch.nn.functional.pad(weight.float(), (0, groups * group_size - K)).view(N, groups, group_size)
+    w = torch.nn.functional.pad(weight.detach().float(), (0, groups * group_size - K)).view(N, groups, group_size)
     largest = w.abs().amax(-1)
     if symmetric:
         exact = largest / 7
