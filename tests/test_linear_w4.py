@@ -273,3 +273,17 @@ def test_quantizing_a_parameter_keeps_no_graph():
             assert (a is None) == (b is None)
             if a is not None:
                 assert not a.requires_grad and a.grad_fn is None and torch.equal(a, b)
+
+
+def test_quantizer_refusals_name_their_reason():
+    w = torch.randn(4, 64, generator=torch.Generator().manual_seed(0))
+    bad = w.clone()
+    bad[1, 3] = float("nan")
+    wide = w.clone()
+    wide[2, 60] = -float("inf")
+    for args, text in ((([1.0],), "expected a Tensor"), ((w[0],), "dimensions"), ((w.double(),), "unsupported_dtype"),
+                       ((w, 48), "unsupported_shape"), ((w, 64.0), "unsupported_shape"), ((w, "64"), "unsupported_shape"),
+                       ((w[:, :40],), "unsupported_shape"), ((w[:, :0],), "unsupported_shape"),
+                       ((bad, 32), "unsupported_value"), ((wide, 32, False), "unsupported_value")):
+        with pytest.raises(RuntimeError, match=text):
+            ops.quantize_linear_w4(*args)

@@ -27,11 +27,15 @@ class W4Weight(NamedTuple):
 def quantize_linear_w4(weight: torch.Tensor, group_size: int = 128, symmetric: bool = True) -> W4Weight:
     """Rounds a [N, K] weight to 4 bits with a scale (and, if not ``symmetric``, a zero point) for each group of
     ``group_size`` values along K. Done once when a model is loaded; plain torch operations on the weight's device."""
+    if not isinstance(weight, torch.Tensor):
+        raise RuntimeError(f"weight is {type(weight).__name__}, expected a Tensor")
     if weight.dim() != 2 or weight.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise RuntimeError(f"unsupported_dtype: weight is {weight.dtype} with {weight.dim()} dimensions")
     N, K = weight.shape
-    if group_size not in GROUP_SIZES or K % 32 != 0 or K == 0:
+    if not isinstance(group_size, int) or group_size not in GROUP_SIZES or K % 32 != 0 or K == 0:
         raise RuntimeError(f"unsupported_shape: K = {K} (a multiple of 32), groups of {group_size} (one of {GROUP_SIZES})")
+    if not bool(torch.isfinite(weight).all()):
+        raise RuntimeError("unsupported_value: weight has infinite values or NaN")
     groups = -(-K // group_size)
     w = torch.nn.functional.pad(weight.detach().float(), (0, groups * group_size - K)).view(N, groups, group_size)
     largest = w.abs().amax(-1)
