@@ -337,3 +337,15 @@ def test_eps_zero_with_groups_that_have_no_row(M, D, dtype):
     for post, pre, has_dz in ((True, True, True), (True, True, False), (False, True, True), (True, False, False)):
         _, r = _check(M, D, dtype, post=post, pre=pre, has_dz=has_dz, eps=0.0, seed=M + D)
         assert all(bool(torch.isfinite(t).all()) for t in r if t is not None)
+
+
+def test_activations_and_eps_of_other_kinds_are_refused():
+    x = torch.zeros(4, 8)
+    for bad in (None, ["silu"], {}):
+        with pytest.raises(RuntimeError, match="unsupported_gate"):
+            ops.run_block_norm(x, gate=x, gate_act=bad)
+    for bad in (None, "small", torch.ones(2)):
+        with pytest.raises(RuntimeError, match="unsupported_eps"):
+            ops.run_block_norm(x, eps=bad)
+        with pytest.raises(RuntimeError, match="unsupported_alpha"):
+            ops.run_block_norm(x, alpha=bad)

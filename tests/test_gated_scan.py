@@ -380,3 +380,20 @@ def test_states_that_are_no_tensors_are_refused():
             ops.run_temporal_gated_scan_backward(x, x, x, bad)
         with pytest.raises(RuntimeError, match="dh_last is"):
             ops.run_temporal_gated_scan_backward(x, x, x, dh_last=bad)
+
+
+@gpu
+def test_outputs_that_are_no_tensors_are_refused():
+    x = torch.zeros(4, 2, 8, device=DEV)
+    for bad in ([0.0], 1.0):
+        with pytest.raises(RuntimeError, match="unsupported_output: h_seq_out"):
+            ops.run_temporal_gated_scan(x, x, h_seq_out=bad)
+        with pytest.raises(RuntimeError, match="unsupported_output: h_last_out"):
+            ops.run_temporal_gated_scan(x, x, h_last_out=bad)
+
+
+def test_gates_of_other_kinds_are_refused():
+    x = torch.zeros(4, 2, 8)
+    for bad in (None, 1, ["sigmoid"], {}):
+        with pytest.raises(RuntimeError, match="unsupported_gate"):
+            ops.run_temporal_gated_scan(x, x, gate=bad)

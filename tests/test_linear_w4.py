@@ -287,3 +287,18 @@ def test_quantizer_refusals_name_their_reason():
                        ((bad, 32), "unsupported_value"), ((wide, 32, False), "unsupported_value")):
         with pytest.raises(RuntimeError, match=text):
             ops.quantize_linear_w4(*args)
+
+
+def test_group_sizes_and_outputs_of_other_kinds_are_refused():
+    x, q, s = torch.zeros(2, 64), torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1)
+    for group in (64.0, "64", None, [64]):
+        with pytest.raises(RuntimeError, match="unsupported_group_size"):
+            ops.run_linear_w4(x, q, s, group_size=group)
+
+
+@gpu
+def test_outputs_that_are_no_tensors_are_refused():
+    x, q, s, _, _ = (_dev(t) for t in _inputs(2, 64, 8, 64, torch.float32, zeros=False, bias=False))
+    for out in ([[0.0] * 8] * 2, 1.0):
+        with pytest.raises(RuntimeError, match="unsupported_output"):
+            ops.run_linear_w4(x, q, s, group_size=64, out=out)

@@ -36,7 +36,14 @@ class BlockNormGradients(NamedTuple):
     dw_pre: Optional[torch.Tensor]
 
 
-def check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm, pre_norm, eps,
+def _number(v) -> Optional[float]:
+    try:
+        return float(v)
+    except (TypeError, ValueError, RuntimeError):       # the last: a tensor of several values
+        return None
+
+
+def check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm, pre_norm, eps, alpha=1.0,
                              **more) -> List[str]:
     """Reasons why the kernel cannot take this call (empty = it can). ``more``: further row tensors by name."""
     name, lead = ("y", y) if y is not None else ("residual", residual)
@@ -50,7 +57,7 @@ def check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_a
     shape, D = lead.shape, int(lead.shape[-1])
     if not 1 <= D <= MAX_D:
         g.add("unsupported_shape", f"rows of {D} values, 1 to {MAX_D} are implemented")
-    if gate_act not in ACTS:
+    if not isinstance(gate_act, str) or gate_act not in ACTS:
         g.add("unsupported_gate", f"gate_act is {gate_act!r}, one of {sorted(ACTS)}")
     elif (gate is None) != (gate_act == "none"):
         g.add("unsupported_gate", f"gate_act is {gate_act!r} {'without a' if gate is None else 'with a'} gate")
@@ -60,8 +67,11 @@ def check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_a
         g.add("unsupported_form", "w_post is given although post_norm is off")
     if w_pre is not None and not pre_norm:
         g.add("unsupported_form", "w_pre is given although pre_norm is off")
-    if not (eps >= 0.0):
+    number = _number(eps)
+    if number is None or not number >= 0.0:
         g.add("unsupported_eps", f"eps is {eps}")
+    if _number(alpha) is None:
+        g.add("unsupported_alpha", f"alpha is {alpha}")
     for n, t in (("gate", gate), ("residual", residual), *more.items()):
         if t is None or t is lead:
             continue
@@ -87,11 +97,12 @@ def check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_a
     return g.why
 
 
-def _is_plain(y, rows, params, gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps) -> bool:
+def _is_plain(y, rows, params, gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps, alpha) -> bool:
     """Whether nothing needs a second look: what ``check_block_norm_support`` would say yes to, at the price that a decoding
     step can pay. Anything else goes through the full check."""
-    if not (type(y) is torch.Tensor and y.is_cuda and y.dim() >= 1 and y.dtype in ACT_DTYPES and eps >= 0.0
-            and (gate is None) == (gate_act == "none") and gate_act in ACTS
+    if not (type(y) is torch.Tensor and y.is_cuda and y.dim() >= 1 and y.dtype in ACT_DTYPES
+            and type(eps) in (float, int) and eps >= 0.0 and type(alpha) in (float, int)
+            and type(gate_act) is str and (gate is None) == (gate_act == "none") and gate_act in ACTS
             and (post_norm or w_post is None) and (pre_norm or w_pre is None)):
         return False
     shape, dtype, device = y.shape, y.dtype, y.device
@@ -144,9 +155,10 @@ def run_block_norm(
     fp32. ``res_inplace`` writes res_out over ``residual``, which must be contiguous and share no
     memory with y or gate then.
     """
-    if not _is_plain(y, (gate, residual), (w_post, res_scale, w_pre), gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps):
+    if not _is_plain(y, (gate, residual), (w_post, res_scale, w_pre), gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps,
+                     alpha):
         raise_reasons("block_norm", check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm,
-                                                             pre_norm, eps), False, verbose)
+                                                             pre_norm, eps, alpha), False, verbose)
     lead = y if y is not None else residual
     if y is None and not pre_norm:
         raise RuntimeError("unsupported_form: neither y nor pre_norm, nothing to compute")
@@ -193,8 +205,9 @@ def run_block_norm_backward(
     order, and None for a parameter that is None.
     """
     if (dres_out is None and dz is None) or (dz is not None and not pre_norm) or not _is_plain(
-            y, (gate, residual, dres_out, dz), (w_post, res_scale, w_pre), gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps):
-        why = check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm, pre_norm, eps,
+            y, (gate, residual, dres_out, dz), (w_post, res_scale, w_pre), gate, w_post, w_pre, gate_act, post_norm, pre_norm, eps,
+            alpha):
+        why = check_block_norm_support(y, gate, residual, w_post, res_scale, w_pre, gate_act, post_norm, pre_norm, eps, alpha,
                                        dres_out=dres_out, dz=dz)
         if dres_out is None and dz is None:
             why.append("unsupported_form: neither dres_out nor dz")

@@ -70,7 +70,7 @@ def check_linear_w4_support(x, q_weight, scales, zeros, bias, group_size) -> Lis
         return g.why
     g.lead_is(rank=x.dim())
     K = int(x.shape[-1])
-    if group_size not in GROUP_SIZES:
+    if not isinstance(group_size, int) or group_size not in GROUP_SIZES:
         g.add("unsupported_group_size", f"groups of {group_size} values, one of {GROUP_SIZES} is implemented")
         return g.why
     if K == 0 or K % 32 != 0:
@@ -104,7 +104,7 @@ def _is_plain(x, q, s, z, b, group_size) -> bool:
     """Whether nothing needs a second look: what ``check_linear_w4_support`` would say yes to, at the price that a decoding
     step can pay. Anything else goes through the full check."""
     if not (type(x) is torch.Tensor and type(q) is torch.Tensor and type(s) is torch.Tensor and x.is_cuda and x.dim() >= 1
-            and q.dim() == 2 and x.dtype in ACT_DTYPES and group_size in GROUP_SIZES):
+            and q.dim() == 2 and x.dtype in ACT_DTYPES and type(group_size) is int and group_size in GROUP_SIZES):
         return False
     K, (N, half), dtype, device = x.shape[-1], q.shape, x.dtype, x.device
     if not (K > 0 and K % 32 == 0 and 2 * half == K and N > 0 and q.dtype == torch.uint8 and s.dtype == dtype
@@ -136,7 +136,7 @@ def run_linear_w4(
     shape = (*x.shape[:-1], N)
     if out is None:
         out = x.new_empty(shape)
-    elif tuple(out.shape) != shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
+    elif not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
         raise RuntimeError(f"unsupported_output: out must be a contiguous {x.dtype} tensor of shape {shape} on {x.device}")
     M = x.numel() // K
     if M > 0:

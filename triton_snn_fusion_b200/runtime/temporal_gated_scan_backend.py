@@ -61,7 +61,7 @@ def check_temporal_gated_scan_support(x_seq, gate_seq, h_init, gate, lengths=Non
     if not g:
         return g.why
     g.lead_is(rank=3)
-    if gate not in GATES:
+    if not isinstance(gate, str) or gate not in GATES:
         g.add("unsupported_gate", f"gate is {gate!r}, one of {sorted(GATES)}")
     if x_seq.dim() == 3:
         _like(g, "gate_seq", gate_seq, x_seq.shape)
@@ -83,7 +83,7 @@ def _is_plain(x, g, gate, h0, lengths, batch_first, state_dtype) -> bool:
     """Whether nothing needs a second look: what ``check_temporal_gated_scan_support`` would say yes to, at the price that a
     decoding step can pay. Anything else goes through the full check."""
     if not (type(x) is torch.Tensor and type(g) is torch.Tensor and x.is_cuda and x.dim() == 3 and x.dtype in ACT_DTYPES
-            and g.shape == x.shape and g.dtype == x.dtype and g.device == x.device and gate in GATES
+            and g.shape == x.shape and g.dtype == x.dtype and g.device == x.device and type(gate) is str and gate in GATES
             and state_dtype in (None, torch.float32)):
         return False
     B, D = x.shape[0 if batch_first else 1], x.shape[2]
@@ -104,7 +104,7 @@ def _strides(t, batch_first):
 def _state_out(name, t, B, D, dtype, x_seq, like=None):
     if t is None:
         return torch.empty_like(like) if like is not None else x_seq.new_empty((B, D), dtype=dtype)
-    if tuple(t.shape) != (B, D) or t.dtype != dtype or t.device != x_seq.device or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or tuple(t.shape) != (B, D) or t.dtype != dtype or t.device != x_seq.device or not t.is_contiguous():
         raise RuntimeError(f"unsupported_output: {name} must be a contiguous {dtype} tensor of shape {(B, D)} on {x_seq.device}")
     return t
 
@@ -148,7 +148,7 @@ def run_temporal_gated_scan(
         h = dense_like(x)
     else:
         h = h_seq_out
-        if h.shape != x.shape or h.dtype != x.dtype or h.device != x.device or (D > 1 and h.stride(2) != 1):
+        if not isinstance(h, torch.Tensor) or h.shape != x.shape or h.dtype != x.dtype or h.device != x.device or (D > 1 and h.stride(2) != 1):
             raise RuntimeError(f"unsupported_output: h_seq_out must be a {x.dtype} tensor of shape {tuple(x.shape)} with "
                                f"dense rows on {x.device}")
     h_last = _state_out("h_last_out", h_last_out, B, D, s_dt, x, h0)
