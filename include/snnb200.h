@@ -343,7 +343,10 @@ int snnb_avgpool_linear_mean(const void *x_seq, const void *fc_w, const void *fc
  *   every SNNB_GATED_SCAN_CKPT_STEPS-th step for the backward pass. T <= SNNB_GATED_SCAN_CKPT_STEPS needs none.
  * T = 1 is the step of a decoder; T = 0 copies the state. T <= 2^30, B * D <= 2^36, and for T > 1 a _t_stride is below
  * 2^29 (SNNB_ERR_UNSUPPORTED otherwise). Gates outside [-1, 1] are taken as they are, but over long
- * sequences the products of such gates may leave the range of fp32 although every h_t stays inside it.
+ * sequences the products of such gates may leave the range of fp32 although every h_t stays inside it. A state that has
+ * become infinite stays infinite or becomes NaN: stretches of steps are joined by the products of their gates, a product
+ * of small gates may be 0 in fp32, and 0 times infinity is NaN. Where that happens depends on how the sequence is split. The
+ * same holds for an infinite gradient on its way to the front. Other channels and the steps before are not touched.
  */
 #define SNNB_GATED_SCAN_CKPT_STEPS 128
 int64_t snnb_gated_scan_ckpt_rows(int64_t T);

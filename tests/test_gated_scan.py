@@ -397,3 +397,30 @@ def test_gates_of_other_kinds_are_refused():
     for bad in (None, 1, ["sigmoid"], {}):
         with pytest.raises(RuntimeError, match="unsupported_gate"):
             ops.run_temporal_gated_scan(x, x, gate=bad)
+
+
+@gpu
+@pytest.mark.parametrize("T", [6, 60, 500, 3000])
+@pytest.mark.parametrize("D", [64, 65])
+def test_an_infinite_state_stays_in_its_channel_and_its_future(T, D):
+    """Small gates, whose products over a tile are 0 in fp32: the state stays infinite or becomes NaN, never a number again;
+    the steps before it and the other channels are those of a clean input, and so for an infinite gradient the other way."""
+    x, gate, _, dh, _ = _inputs(T, 2, D, torch.float32, "sigmoid", carry=False)
+    x, gate, dh = x.to(DEV), (gate - 5).to(DEV), dh.to(DEV)
+    clean = ops.run_temporal_gated_scan(x, gate, save_for_backward=True)
+    t = T // 2
+    x2 = x.clone()
+    x2[t, 1, 5] = float("inf")
+    h = ops.run_temporal_gated_scan(x2, gate).h_seq
+    assert not bool(torch.isfinite(h[t:, 1, 5]).any()) and float(h[t, 1, 5]) == float("inf")
+    h[t:, 1, 5] = clean.h_seq[t:, 1, 5]
+    assert torch.equal(h, clean.h_seq)
+    want = ops.run_temporal_gated_scan_backward(dh, x, gate, None, clean.ckpt)
+    dh2 = dh.clone()
+    dh2[t, 1, 5] = -float("inf")
+    got = ops.run_temporal_gated_scan_backward(dh2, x, gate, None, clean.ckpt)
+    assert not bool(torch.isfinite(got.dx[:t + 1, 1, 5]).any()) and not bool(torch.isfinite(got.dh_init[1, 5]))
+    got.dx[:t + 1, 1, 5] = want.dx[:t + 1, 1, 5]
+    got.dgate[:t + 1, 1, 5] = want.dgate[:t + 1, 1, 5]
+    got.dh_init[1, 5] = want.dh_init[1, 5]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

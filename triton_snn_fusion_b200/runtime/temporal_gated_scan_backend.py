@@ -132,7 +132,8 @@ def run_temporal_gated_scan(
     are neither read nor counted, their h_seq is zero. ``h_seq_out`` / ``h_last_out``: tensors to write into;
     ``h_last_out`` may be ``h_init`` itself (a decoder's state updated in place); otherwise they share no memory with the
     inputs or each other. Rows may be parts of wider ones (x and
-    gate as two halves of one projection); an innermost dimension that is not dense is copied first.
+    gate as two halves of one projection); an innermost dimension that is not dense is copied first. The gates have x_seq's
+    type. A state that has become infinite stays infinite or becomes NaN, in its channel alone.
     """
     if not _is_plain(x_seq, gate_seq, gate, h_init, lengths, batch_first, state_dtype):
         raise_reasons("temporal_gated_scan",
