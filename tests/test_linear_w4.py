@@ -302,3 +302,10 @@ def test_outputs_that_are_no_tensors_are_refused():
     for out in ([[0.0] * 8] * 2, 1.0):
         with pytest.raises(RuntimeError, match="unsupported_output"):
             ops.run_linear_w4(x, q, s, group_size=64, out=out)
+
+
+@gpu
+def test_the_microbenchmark_rotates_weights_that_fit_the_cache(capsys):
+    from triton_snn_fusion_b200 import microbench
+    microbench.main(["w4", "--M", "2", "--K", "4096", "--N", "8192"])       # 16.8 MB of weights: 25 of them are 400 MB
+    assert "(25 rotating weights)" in capsys.readouterr().out

@@ -78,14 +78,18 @@ def case_conv(a):
           f"spike rate {float(sp.float().mean()):.3f}  device status {_lib.device_status()}")
 
 
+def _copies(footprint):
+    """Footprints below the L2 size would be served from L2 on every repetition: rotate through enough copies of the
+    buffers that a launch never finds its data cached (every copy holds different seeded values)."""
+    return max(1, -(-(400 << 20) // footprint)) if footprint < (256 << 20) else 1
+
+
 def case_lif(a):
     dt = {"f32": torch.float32, "bf16": torch.bfloat16}[a.dtype]
     dc = _lib.dtype_code(dt)
     es = 4 if a.dtype == "f32" else 2
-    # Footprints below the L2 size would be served from L2 on every repetition: rotate through enough copies of the
-    # buffers that a launch never finds its data cached (every copy holds different seeded values).
     footprint = es * (2 * a.T + 1) * a.n
-    copies = max(1, -(-(400 << 20) // footprint)) if footprint < (256 << 20) else 1
+    copies = _copies(footprint)
     g = torch.Generator(device=DEV).manual_seed(0)
     xs = [(torch.randn(a.T, a.n, device=DEV, generator=g) * 0.8 + 0.6).to(dt) for _ in range(copies)]
     sps = [torch.empty_like(x) for x in xs]
@@ -235,12 +239,19 @@ def case_norm(a):
 def case_w4(a):
     from .runtime.linear_w4_backend import quantize_linear_w4, run_linear_w4
     g = torch.Generator(device=DEV).manual_seed(0)
-    q = quantize_linear_w4(torch.randn(a.N, a.K, device=DEV, generator=g).to(DTYPES[a.dtype]), a.group)
+    copies = min(64, _copies(a.N * a.K // 2))
+    qs = [quantize_linear_w4(torch.randn(a.N, a.K, device=DEV, generator=g).to(DTYPES[a.dtype]), a.group) for _ in range(copies)]
     x = torch.randn(a.M, a.K, device=DEV, generator=g).to(DTYPES[a.dtype])
-    ms = _time(lambda: run_linear_w4(x, *q, group_size=a.group), a.reps)
-    nbytes = a.N * a.K / 2 + q.scales.numel() * q.scales.element_size() + (x.numel() + a.M * a.N) * x.element_size()
+    k = [0]
+
+    def call():
+        k[0] += 1
+        run_linear_w4(x, *qs[k[0] % copies], group_size=a.group)
+
+    ms = _time(call, max(a.reps, 2 * copies) if a.reps > 1 else 1)
+    nbytes = a.N * a.K / 2 + qs[0].scales.numel() * qs[0].scales.element_size() + (x.numel() + a.M * a.N) * x.element_size()
     print(f"linear_w4 M{a.M} {a.K}->{a.N} G{a.group} {a.dtype}: {ms:.4f} ms  {nbytes / ms / 1e6:.0f} GB/s  "
-          f"{2.0 * a.M * a.N * a.K / ms / 1e9:.1f} TFLOP/s")
+          f"{2.0 * a.M * a.N * a.K / ms / 1e9:.1f} TFLOP/s  ({copies} rotating weights)")
 
 
 def case_mma(a):
