@@ -412,8 +412,8 @@ int snnb_block_norm_backward(const void *dres_out, int64_t dres_out_stride, cons
  *   y[m][n] = sum_k x[m][k] * (q[n][k] - zero[n][k / G]) * scale[n][k / G] + bias[n],   G = group_size
  *   x [M][K] (rows x_stride elements apart), q_weight [N][K / 2] bytes, 16-byte aligned: weight k in the low (k even) or
  *   high (k odd) half of byte k / 2; scales [N][ceil(K / G)] and bias [N] (or NULL) in the x dtype; zeros
- *   [N][ceil(K / G)] uint8, at most 127 (a larger one makes its column of y NaN for bf16 and fp32 tokens), or NULL (8
- *   everywhere); y [M][N], rows y_stride elements apart, apart from x.
+ *   [N][ceil(K / G)] uint8, at most 127 (a larger one makes its column of y infinite or NaN for bf16 and fp32 tokens),
+ *   or NULL (8 everywhere); y [M][N], rows y_stride elements apart, apart from x.
  * K % 32 == 0, G 32, 64 or 128; the last group may be shorter than G. K <= 2^30, N * K < 2^33, M <= 131070. The weights are read
  * once for every 32 tokens (fp32: 10), so beyond some hundred tokens a product over widened weights is the faster way.
  */

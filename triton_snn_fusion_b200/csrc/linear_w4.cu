@@ -65,10 +65,15 @@ template <typename H> __device__ __forceinline__ void unpack8(uint32_t w, const 
     for (int i = 0; i < 4; ++i) p[i] = minus<H>(and_or(w >> (4 * i), 0x000f000fu, magic<H>()), zero[0]);
   }
 }
-// The two constants of unpack8 for a zero point. Beyond 127, magic + zero is no bf16 number any more: that makes the weights
-// NaN rather than wrong.
-template <typename H> __device__ __forceinline__ void zeros_of(uint32_t z, uint32_t (&zero)[2]) {
-  zero[0] = !std::is_same_v<H, __half> && z > 127 ? 0x7fff7fffu : magic<H>() + 0x00010001u * z;
+// The two constants of unpack8 for a zero point (ZERO: any may come, else it is 8). Beyond 127, magic + zero is no bf16 number
+// any more: the byte's sign, copied beside it, then makes it infinite or NaN, and with it the products, rather than wrong.
+template <typename H, bool ZERO> __device__ __forceinline__ void zeros_of(uint32_t z, uint32_t (&zero)[2]) {
+  if constexpr (ZERO && !std::is_same_v<H, __half>) {
+    asm("prmt.b32 %0, %1, 0, 0x8080;" : "=r"(zero[0]) : "r"(z));
+    zero[0] |= magic<H>();
+  } else {
+    zero[0] = magic<H>() + 0x00010001u * z;
+  }
   if constexpr (std::is_same_v<H, __half>) {      // -(64 + z): 64 .. 127 have steps of 1/16 in fp16, beyond that of 1/8
     const __half2 v = __half2half2(__int2half_rn(-64 - (int)z));
     zero[1] = *reinterpret_cast<const uint32_t *>(&v);
@@ -279,7 +284,7 @@ __global__ void __launch_bounds__(kWarps * 32) linear_w4_kernel(const __grid_con
             for (int r = 0; r < 2; ++r) {
               uint32_t z;
               sc[i][t][r].get((lane & ~3) | h, scale[t][r], z);
-              zeros_of<H>(z, zero[t][r]);
+              zeros_of<H, ZERO>(z, zero[t][r]);
             }
 #pragma unroll
           for (int v = 0; v < WORDS; ++v) {

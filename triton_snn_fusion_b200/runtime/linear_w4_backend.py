@@ -129,7 +129,7 @@ def run_linear_w4(
 ) -> torch.Tensor:
     """x [..., K] -> [..., N] in x's dtype. ``q_weight``, ``scales`` and ``zeros`` as ``quantize_linear_w4`` lays them out;
     keep them contiguous (they are copied at every call otherwise). A zero point above 127, which no 4-bit weight needs, makes
-    its output NaN for bf16 and fp32 tokens. ``out``: a contiguous tensor to write into, apart from x."""
+    its output infinite or NaN for bf16 and fp32 tokens. ``out``: a contiguous tensor to write into, apart from x."""
     if not _is_plain(x, q_weight, scales, zeros, bias, group_size):
         raise_reasons("linear_w4", check_linear_w4_support(x, q_weight, scales, zeros, bias, group_size), False, verbose)
     K, N = int(x.shape[-1]), int(q_weight.shape[0])
