@@ -16,11 +16,12 @@
 //
 // What bounds it, on B200: forward 5 values an element (read y, gate, res; write res', z), backward 8. A block takes whole
 // rows, 8 (16-bit) or 4 columns a thread, one after the other; the next rows are copied into shared memory meanwhile. 16384
-// rows of 2048 bf16 values, in us: forward 60 = 5.5 TB/s (85 % of the measured copy rate; three rows in shared memory
-// instead of two 68, the next row in registers 90), backward 113 with its sums = 4.7 TB/s (72 %): 60 instructions an
-// element, a third of them the four sums over a row, at two blocks an SM for its 126 registers (three blocks of 80 with
-// spills 160, rows in registers instead of shared memory 181). Gradients of the parameters leave as one row per block and
-// are joined in a fixed order by a second kernel, which costs 4 us; nothing is summed by atomics.
+// rows of 2048 bf16 values, device time in us: forward 55 = 6.1 TB/s (93 % of the measured copy rate; a call alone with cold
+// caches 60, three rows in shared memory instead of two 68, the next row in registers 90), backward 104 with its sums = 5.1
+// TB/s (78 %; alone 113); 1024 fp32 columns 57 and 104. The backward pass: 60 instructions an element, a third of them the
+// four sums over a row, at two blocks an SM for its 123 registers (three blocks of 80 with spills 160, rows in registers
+// instead of shared memory 181). Gradients of the parameters leave as one row per block and are joined in a fixed order by a
+// second kernel, which costs 4 us; nothing is summed by atomics.
 #include "packed.cuh"
 #include "umma.cuh"
 
@@ -723,8 +724,8 @@ __global__ void __launch_bounds__(1024) block_norm_sums_kernel(const __grid_cons
 // How the rows are laid over threads. One piece of 16 bytes a thread: with two and half the threads the forward pass took
 // 70 us instead of 61 (16384 rows of 2048 bf16 values), and the backward pass has no registers for them. Two pieces only
 // where 512 threads with one do not reach (up to 8192 16-bit or 4096 fp32 columns), single columns where rows do not start
-// on 16-byte boundaries (4096 rows of 2047 bf16 values: forward 2.4 TB/s, backward 1.1; loading a row ahead into registers
-// changed nothing), and the long-row kernel (1.1 TB/s backward at 16384 columns, rows being read five times) behind that.
+// on 16-byte boundaries (4096 rows of 2047 bf16 values: forward 29 us = 2.9 TB/s, backward 79 us = 1.7), and the long-row
+// kernel (1.1 TB/s backward at 16384 columns, rows being read five times) behind that.
 // A plan: `vec` columns in `nv` pieces for each of tpr threads; nv = 0: the long-row kernel.
 struct Plan { int vec, nv, tpr, threads; };
 Plan plan_of(int D, int dtype, bool aligned) {
@@ -739,10 +740,17 @@ Plan plan_of(int D, int dtype, bool aligned) {
   return p;
 }
 
-// Blocks of the backward pass, each of which leaves one row of column sums: as many as run at once on 148 SMs. The same for
-// every type and alignment, so that the workspace depends on the sizes alone. Measured, us for 1, 2, 3, 4, 6, 8 blocks an SM
-// (bf16): 65536 rows of 128 51 40 38 45 42 46; 32768 of 512 177 99 81 67 63 77; 16384 of 1024 102 72 66 78 72 80; 16384 of
-// 2048 145 114 128 122 131 140; 8192 of 4096 137 143 154 164 182 201.
+// Blocks of the backward pass, each of which leaves one row of column sums: the same for every type and alignment, so that
+// the workspace depends on the sizes alone, and chosen for 16-bit rows on 16-byte boundaries. Device time in us for 1, 2, 3,
+// 4, 6, 8 blocks an SM (the choice in brackets):
+//   bf16    65536 x 128    45 32 [29] 28 34 33      fp32    32768 x 256   136 74 [59] 50 50 55
+//           32768 x 512    171 92 75 61 [54] 54             16384 x 512   79 52 48 52 [57] 54
+//           16384 x 1024   95 63 [56] 54 64 61              16384 x 1024  106 95 [106] 93 94 96
+//           16384 x 2048   136 [104] 118 113 120 131        8192 x 2048   95 [99] 103 111 121 125
+//           8192 x 4096    [125] 135 142 151 167 182        1023 x 1001   18.5 15.6 [17.5] 17.8 20.2 21.5
+//           1024 x 16384   241 [252] 262 268 284 290
+//   ragged bf16  65536 x 63  103 58 [44] 37 48 41   16384 x 333  185 99 71 58 [75] 60   8192 x 1001  109 65 [84] 68 73 74
+//                4096 x 2047  75 [78] 82 83 89 95
 int backward_blocks(int64_t M, int D) {
   const int most = 148 * (D <= 256 ? 3 : D <= 512 ? 6 : D <= 1024 ? 3 : D <= 2048 ? 2 : D <= 8192 ? 1 : 2);
   return (int)(M < most ? (M < 1 ? 1 : M) : most);

@@ -11,11 +11,12 @@
 // atomics, so a result depends on the split (which depends on the sizes and the number of SMs alone) but not on the run.
 //
 // What bounds it, on B200: forward 6, backward 10 bytes an element (bf16) at the floor. B8 T2048 D2048 bf16, 33.5 M
-// elements: forward 47 us = 4.3 TB/s (65 % of the measured copy rate), backward about 75 us = 4.5 TB/s. An element costs 19
-// instructions forward, two of them on the special-function pipe, and the 512 blocks leave every seventh place of the
-// GPU's 592 empty: issue slots and that imbalance are what is left (issue 52 % of the active cycles, SMs active 78 % of
-// the time). The packed fp32 instructions, the joiners (instead of every thread folding the maps in front of it: 128
-// registers and spills, 71 us) and the copies past L1 are what brought it there from 195 us.
+// elements, device time: forward 39 us = 5.1 TB/s (78 % of the measured copy rate), backward 70 us = 4.8 TB/s (73 %); the
+// same in fp32 with D1024 39 and 69, padded batches of half as many steps 33 and 57. An element costs 19 instructions
+// forward, two of them on the special-function pipe, and the 512 blocks leave every seventh place of the GPU's 592 empty:
+// issue slots and that imbalance are what is left (issue 51 % of the active cycles). The packed fp32 instructions, the
+// joiners (instead of every thread folding the maps in front of it: 128 registers and spills, 71 us) and the copies past L1
+// are what brought it there from 195 us.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -691,9 +692,9 @@ int launch_tiles(ScanArgs q, int threads, int CH, int S, int smem, cudaStream_t 
 //   B2 T4096 D2048 (128)            34 29 24 27 / 62 49 52 51       B1 T1024 D4096    10.3 10.1 8.9 11.2 / 17 15 17 18
 //   B4 T2048 D2048 (256)            24 23 25 29 / 42 40 48 55       B16 T1024 D1024 (512)   21 25 28 37 / 37 40 49 64
 //   B2 T16384 D512 (32)             126 85 44 31 / 238 147 75 50
-// The ragged backward kernel (512 threads, two blocks an SM) is given as many blocks as two rounds take, its loads being
+// The ragged backward kernel (512 threads, two blocks an SM) is given as many blocks as two waves take, its loads being
 // what it waits for: B2 T4096 D2047 (128 tiles) 188 131 110 105, B1 T8192 D2047 (64) 361 203 131 116, B4 T2048 D2047 (256)
-// 120 105 100 107; at short sequences one round is a little better: B1 T1024 D2047 38 23 17 18, B6 T1031 D1001 fp32 (192)
+// 120 105 100 107; at short sequences one wave is a little better: B1 T1024 D2047 38 23 17 18, B6 T1031 D1001 fp32 (192)
 // 51 53 55 75.
 int scan_cluster(int64_t tiles, int64_t steps, int CH, int most, int smem) {
   const int sms = sm_count() > 0 ? sm_count() : 148;
@@ -707,6 +708,7 @@ int scan_cluster(int64_t tiles, int64_t steps, int CH, int most, int smem) {
 }
 
 // Up to 8 steps a thread walks alone. Beyond that:
+// (The figures below are single calls, timed in steps of about 2 us.)
 // - rows on 16-byte boundaries, up to 64 steps: one tile, no longer than needed, through shared memory. Measured against
 //   the tile of 32 steps straight to registers and, from 33 steps on, the tile of 128 (bf16, D2048, us, forward and
 //   backward): T16 B256 23 43 instead of 41 64, T24 B160 25 41 instead of 31 45, T33 B128 33 49 instead of 51 80, T64 B64

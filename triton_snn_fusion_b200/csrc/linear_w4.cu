@@ -35,8 +35,8 @@ struct W4Args {
 template <typename T> struct Half16 { using type = T; };
 template <> struct Half16<float> { using type = __nv_bfloat16; };      // fp32 tokens: three bf16 pieces, see pieces_of
 
-// Two weights as two 16-bit floats: magic + q has q in its lowest bits (1024 + q in fp16, 128 + q in bf16), and
-// subtracting magic + zero is exact.
+// Two weights as two 16-bit floats, the well-known way by the bits of a larger number: magic + q has q in its lowest bits
+// (1024 + q in fp16, 128 + q in bf16), and subtracting magic + zero is exact.
 template <typename H> __device__ __forceinline__ uint32_t magic() { return std::is_same_v<H, __half> ? 0x64006400u : 0x43004300u; }
 template <typename H> __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -378,7 +378,7 @@ template <typename T, bool ZERO, int G, int NT, int RT, int DEPTH> int go(const 
 // and with (RT, DEPTH) = (2, 2) (2, 1) (4, 1), 32 tokens 8192 -> 8192 37 38 27, 64 tokens 4096 -> 8192 40 41 29.
 // More rows a warp share what a step costs beside the weights; fewer blocks than twice the SMs cost more than that. With two
 // tiles a block three blocks run on an SM (65 registers; 111 and two blocks with two steps ahead), so that up to six tiles an
-// SM are one round.
+// SM are one wave.
 template <typename T, bool ZERO, int G> int by_tokens(const W4Args &a, cudaStream_t s) {
   const int cols = (int)(a.M < 64 ? a.M : 64) * kPieces<T>, tiles = (a.N + 15) / 16, sms = sm_count() > 0 ? sm_count() : 148;
   if (cols > 16) return go<T, ZERO, G, 4, 4, 1>(a, s);
