@@ -424,3 +424,29 @@ def test_an_infinite_state_stays_in_its_channel_and_its_future(T, D):
     got.dgate[:t + 1, 1, 5] = want.dgate[:t + 1, 1, 5]
     got.dh_init[1, 5] = want.dh_init[1, 5]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("T,B,D", [(0, 2, 8), (5, 0, 8), (5, 2, 0), (200, 0, 8), (0, 0, 0)])
+@pytest.mark.parametrize("batch_first", [True, False])
+def test_empty_sizes(T, B, D, batch_first):
+    """Nothing to compute: outputs of the right shapes, and without a step the state is handed on."""
+    x = torch.randn((B, T, D) if batch_first else (T, B, D), device=DEV)
+    h0, dl = torch.randn(B, D, device=DEV), torch.randn(B, D, device=DEV)
+    f = ops.run_temporal_gated_scan(x, x, h0, batch_first=batch_first, save_for_backward=True)
+    assert f.h_seq.shape == x.shape and f.h_last.shape == (B, D)
+    r = ops.run_temporal_gated_scan_backward(x, x, x, h0, f.ckpt, dh_last=dl, batch_first=batch_first)
+    assert r.dx.shape == x.shape and r.dgate.shape == x.shape and r.dh_init.shape == (B, D)
+    if T == 0:
+        assert torch.equal(f.h_last, h0) and torch.equal(r.dh_init, dl)
+    n = torch.zeros(B, dtype=torch.int32, device=DEV)
+    f = ops.run_temporal_gated_scan(x, x, h0, batch_first=batch_first, lengths=n)
+    assert torch.equal(f.h_last, h0) and not bool(f.h_seq.any())
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 61])
+def test_one_step_of_a_padded_batch(D):
+    """A decoding step in which some sequences have ended: their state stays and their row is zero."""
+    _check(1, 5, D, torch.bfloat16, "sigmoid", True, lengths=[1, 0, 1, 0, 3], batch_first=True)
+    _check(1, 5, D, torch.float32, "value", False, lengths=[0, 0, 1, -1, 1])
