@@ -344,7 +344,7 @@ def test_activations_and_eps_of_other_kinds_are_refused():
     for bad in (None, ["silu"], {}):
         with pytest.raises(RuntimeError, match="unsupported_gate"):
             ops.run_block_norm(x, gate=x, gate_act=bad)
-    for bad in (None, "small", torch.ones(2)):
+    for bad in (None, "small", "0.5", torch.ones(2)):
         with pytest.raises(RuntimeError, match="unsupported_eps"):
             ops.run_block_norm(x, eps=bad)
         with pytest.raises(RuntimeError, match="unsupported_alpha"):

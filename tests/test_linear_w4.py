@@ -309,3 +309,11 @@ def test_the_microbenchmark_rotates_weights_that_fit_the_cache(capsys):
     from triton_snn_fusion_b200 import microbench
     microbench.main(["w4", "--M", "2", "--K", "4096", "--N", "8192"])       # 16.8 MB of weights: 25 of them are 400 MB
     assert "(25 rotating weights)" in capsys.readouterr().out
+
+
+def test_a_group_size_may_be_any_whole_number_type():
+    import numpy as np
+    w = torch.randn(4, 64, generator=torch.Generator().manual_seed(0))
+    assert all(torch.equal(a, b) for a, b in zip(ops.quantize_linear_w4(w, np.int64(32), False), ops.quantize_linear_w4(w, 32, False)))
+    with pytest.raises(RuntimeError, match="unsupported_device"):       # and nothing else
+        ops.run_linear_w4(w, *ops.quantize_linear_w4(w, 32), group_size=np.int32(32))

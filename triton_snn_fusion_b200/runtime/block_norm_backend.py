@@ -38,7 +38,7 @@ class BlockNormGradients(NamedTuple):
 
 def _number(v) -> Optional[float]:
     try:
-        return float(v)
+        return None if isinstance(v, str) else float(v)
     except (TypeError, ValueError, RuntimeError):       # the last: a tensor of several values
         return None
 

@@ -8,6 +8,7 @@ Every call that is refused raises a ``RuntimeError`` that names the reason.
 """
 from __future__ import annotations
 
+from numbers import Integral
 from typing import List, NamedTuple, Optional
 
 import torch
@@ -32,10 +33,11 @@ def quantize_linear_w4(weight: torch.Tensor, group_size: int = 128, symmetric: b
     if weight.dim() != 2 or weight.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise RuntimeError(f"unsupported_dtype: weight is {weight.dtype} with {weight.dim()} dimensions")
     N, K = weight.shape
-    if not isinstance(group_size, int) or group_size not in GROUP_SIZES or K % 32 != 0 or K == 0:
+    if not isinstance(group_size, Integral) or group_size not in GROUP_SIZES or K % 32 != 0 or K == 0:
         raise RuntimeError(f"unsupported_shape: K = {K} (a multiple of 32), groups of {group_size} (one of {GROUP_SIZES})")
     if not bool(torch.isfinite(weight).all()):
         raise RuntimeError("unsupported_value: weight has infinite values or NaN")
+    group_size = int(group_size)
     groups = -(-K // group_size)
     w = torch.nn.functional.pad(weight.detach().float(), (0, groups * group_size - K)).view(N, groups, group_size)
     largest = w.abs().amax(-1)
@@ -70,7 +72,7 @@ def check_linear_w4_support(x, q_weight, scales, zeros, bias, group_size) -> Lis
         return g.why
     g.lead_is(rank=x.dim())
     K = int(x.shape[-1])
-    if not isinstance(group_size, int) or group_size not in GROUP_SIZES:
+    if not isinstance(group_size, Integral) or group_size not in GROUP_SIZES:
         g.add("unsupported_group_size", f"groups of {group_size} values, one of {GROUP_SIZES} is implemented")
         return g.why
     if K == 0 or K % 32 != 0:
@@ -147,5 +149,5 @@ def run_linear_w4(
         z = zeros.contiguous() if zeros is not None else None
         b = bias.contiguous() if bias is not None else None
         launch("snnb_linear_w4", x.device, x2.data_ptr(), x2.stride(0), w.data_ptr(), s.data_ptr(), _lib.ptr(z),
-               _lib.ptr(b), out.data_ptr(), N, M, K, N, group_size, _lib.dtype_code(x.dtype))
+               _lib.ptr(b), out.data_ptr(), N, M, K, N, int(group_size), _lib.dtype_code(x.dtype))
     return out
